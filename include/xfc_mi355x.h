@@ -280,6 +280,67 @@ int xfc_topk_scratch(const void* X, int64_t ldx, const void* W, int64_t ldw,
 size_t xfc_layer_workspace_bytes(int64_t max_batch, int64_t L, int64_t d, int64_t max_nnz);
 
 /*
+ * A label matrix in microscaled 4-bit floating point (MX4), for scoring with a quarter of fp16's bytes.  No counterpart in
+ * the reference.  32 consecutive dims of a label share a scale byte s: a weight is 2^(s - 127) times one of +-0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * (4-bit code: sign, two exponent bits, one mantissa bit), s - 127 = floor(log2 of the block's largest magnitude) - 2, at least -127.  Weights
+ * are rounded to the nearest, ties to an even mantissa; what lies above 6 becomes 6.  A block that holds an infinity or a NaN
+ * has s = 255 and stands for NaNs.
+ *   codes:  xfc_mx4_code_bytes(L, d) bytes, [unit][step][tile 4][row 16][block 4][16]: units of 64 labels, steps of 128 dims (of the last one
+ *           as many blocks as the width has); the even dim of two is in a byte's lower half; row 4 q + r of tile 2 p + t is label
+ *           32 p + 8 q + 4 t + r of the unit (p, t < 2, q, r < 4)
+ *   scales: xfc_mx4_scale_bytes(L, d) bytes, [unit][step][block 4][row 16][tile 4]; those of no block have to be 0
+ * Both 16-byte aligned.  The labels behind the last are written as zeros.  W: `type` elements, rows of d with leading dimension ldw; d a multiple of 8,
+ * rows 16-byte aligned.
+ */
+enum xfc_type { XFC_F16 = 0, XFC_BF16 = 1, XFC_F32 = 2 };
+size_t xfc_mx4_code_bytes(int64_t L, int64_t d);
+size_t xfc_mx4_scale_bytes(int64_t L, int64_t d);
+int xfc_mx4_quantize(const void* W, int type, int64_t ldw, int64_t L, int64_t d, void* codes, void* scales, void* stream);
+/* ... and back, rounded once to `type`. */
+int xfc_mx4_dequantize(const void* codes, const void* scales, int64_t L, int64_t d, void* W, int type, int64_t ldw, void* stream);
+
+/*
+ * xfc_logits with an MX4 label matrix: out[B x L] (fp16) = X . W^T.  X (fp16, bf16 or fp32, rows 16-byte aligned) is quantised on its way, in blocks of 32
+ * dims as above: embed_bits 4, to the same numbers, or 8, to a sign, four exponent and three mantissa bits (up to 448,
+ * s - 127 = floor(log2 of the largest) - 8).  Sums in fp32: exact with 4 bits unless scales lie far apart; with 8 bits the matrix pipe drops
+ * what is below some 2^-14 of the largest of neighbouring products.  A block of X with an infinity or a NaN makes its row NaN.
+ * ldo a multiple of 8, out 16-byte aligned.  XFC_ERR_LIMIT: widths above 16,384 (embed_bits 8: 9,088), or more than 2^30 labels.
+ */
+int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, const void* scales, void* out, int64_t ldo,
+                   int64_t B, int64_t L, int64_t d, int embed_bits, void* stream);
+
+/*
+ * xfc_topk with an MX4 label matrix, with the same order of ties, places without a score and clamp to numy.  K <= 8: by the fp32 sums, no logits
+ * are written; 8 < K <= 8192: by the logits of xfc_mx4_logits.  Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, K); with
+ * K > 8 and more than 256 rows what 256 rows take is enough, the rows then go in turns.
+ */
+size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K);
+int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,
+                 int64_t numy, int K, int embed_bits, float* values, int64_t* indices, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Preference loss over P pairs of labels.  Pair p of row b (rowptr[b] <= p < rowptr[b + 1]; int32) says that label chosen[p] is better than
+ * rejected[p] for X[b]:
+ *   margin[p] = X[b] . (W[chosen] - W[rejected]) - reference[p]      (a softmax's log pi(chosen) - log pi(rejected), less the same of
+ *                                                                    a frozen reference: the normalisers cancel)
+ *   loss = sum weight[p] * (-(1 - smoothing) log sigmoid(beta margin) - smoothing log sigmoid(-beta margin))       (one float)
+ *   slope[p] = d loss / d margin = weight[p] * beta * (sigmoid(beta margin) - (1 - smoothing))
+ * and its gradient, in either form or both:
+ *   dX[b] = scale * sum slope[p] (W[chosen] - W[rejected])           (rows of d, dx_type; rows without pairs are written as zero)
+ *   G[b][chosen] += slope[p], G[b][rejected] -= slope[p]             (fp16, as xfc_fwd_grad_* leaves it: xfc_dx and xfc_dw_* then
+ *                                                                    carry the pairs too; entries of one row and label are added up in fp32
+ *                                                                    and rounded once per 512 pairs of the row)
+ * X: fp16, bf16 or fp32.  W: fp16 rows, or with scales non-NULL MX4 codes (ldw is not used).  reference, weight, margin, dX, G may be NULL
+ * (0, 1, not wanted).  A pair with a label outside [0, L) or weight 0 is not there, whatever else it holds: its margin is 0, and so is
+ * that of pairs which no row has.  Results do not depend on anything but the arguments: no atomics.  d <= 4096, a multiple of 8.
+ */
+size_t xfc_preference_workspace_bytes(int64_t B, int64_t P, int64_t d);
+int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t ldw, const void* scales, int64_t L, int64_t d,
+                   const int32_t* rowptr, const int32_t* chosen, const int32_t* rejected, const float* reference, const float* weight,
+                   int64_t B, int64_t P, float beta, float smoothing, float scale, float* loss, float* margin,
+                   void* dX, int dx_type, int64_t lddx, void* G, int64_t ldg, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Plain device-to-device copy of `bytes` bytes (a multiple of 16, 16-byte aligned
  * pointers).  No counterpart in the reference: it is the kernel of known size against
  * which the HBM traffic counters (FETCH_SIZE / WRITE_SIZE) of the other kernels are

@@ -1,0 +1,302 @@
+// Narrow label matrices and label preferences: the C entry points of mx4.hpp and preference.hpp.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/xfc_mi355x.h"
+#include "launch.hpp"
+#include "mx4.hpp"
+#include "preference.hpp"
+
+using namespace xfc;
+
+namespace {
+
+bool type_ok(int t) { return t == XFC_F16 || t == XFC_BF16 || t == XFC_F32; }
+// A row stride in elements, and whether rows of that type can be read in 16-byte pieces.
+bool rows_ok(const void* p, int type, int64_t ld) { return aligned16(p) && ld % (16 / type_bytes(type)) == 0; }
+
+// Calls f with XFC_F16, XFC_BF16 or XFC_F32 as a constant.
+template <class Fn>
+int by_type(int type, Fn&& f) {
+  if (type == XFC_F32) return f(std::integral_constant<int, XFC_F32>{});
+  if (type == XFC_BF16) return f(std::integral_constant<int, XFC_BF16>{});
+  return f(std::integral_constant<int, XFC_F16>{});
+}
+
+int check_mx(const void* W, int type, int64_t ldw, int64_t L, int64_t d, const void* codes, const void* scales, bool& empty) {
+  empty = false;
+  if (!dims_ok(L) || !dims_ok(d) || !type_ok(type)) return XFC_ERR_INVALID;
+  if (L == 0) { empty = true; return XFC_OK; }
+  if (d == 0 || !W || !codes || !scales) return XFC_ERR_INVALID;
+  if (d % 8 || !rows_ok(W, type, ldw) || !aligned16(codes) || !aligned16(scales)) return XFC_ERR_ALIGN;
+  if (ldw < d) return XFC_ERR_SHAPE;
+  if (ceil_div(L, MX_UNIT) * (int64_t)mx_steps(d) > 0x7fffffff) return XFC_ERR_INVALID;
+  return XFC_OK;
+}
+
+// How a product is cut.  Rows: tiles of 16, 32, 64 or 128, as many as the batch fills and the LDS holds.  Label units: dealt to the waves
+// of every workgroup of a row tile.
+struct MxPlan {
+  int nt;              // tiles of 16 rows of a workgroup; 0: the width does not fit
+  int tiles_m, slots;
+  int64_t lds;
+};
+int64_t mx_lds_of(int nt, bool x8, int64_t d) {
+  const int64_t frag = x8 ? MxRows<true>::FRAG : MxRows<false>::FRAG;
+  return (int64_t)mx_steps(d) * (nt * frag + (nt + 3) / 4 * 256);
+}
+MxPlan mx_plan(int64_t rows, int64_t L, int64_t d, bool x8, int run, int cus) {
+  MxPlan p = {};
+  for (p.nt = 8; p.nt > 0; p.nt /= 2) {
+    const int64_t room = p.nt >= 4 ? FULL_LDS : FULL_LDS / 2;
+    if (mx_lds_of(p.nt, x8, d) <= room && (p.nt == 1 || rows > 8 * p.nt)) break;
+  }
+  if (p.nt == 0) {
+    p.nt = 1;  // one workgroup to a CU
+    if (mx_lds_of(1, x8, d) > FULL_LDS) { p.nt = 0; return p; }
+  }
+  p.lds = mx_lds_of(p.nt, x8, d);
+  p.tiles_m = ceil_div(rows, 16 * p.nt);
+  const int per_xcd = (p.nt >= 4 || 2 * p.lds > FULL_LDS ? 1 : 2) * (cus / 8 > 0 ? cus / 8 : 1);
+  const int most = ceil_div(ceil_div(L, MX_UNIT), 8 * MX_WAVES * run);  // workgroups of an XCD that have anything to do
+  p.slots = per_xcd / p.tiles_m;
+  if (p.slots > most) p.slots = most;
+  if (p.slots < 1) p.slots = 1;
+  return p;
+}
+
+// A kernel whose LDS goes by the call: the limit is raised to all there is.
+template <auto Kernel, class A>
+int launch_lds(dim3 g, dim3 b, int64_t lds, hipStream_t st, const A& args) {
+  const hipError_t e = raise_lds_limit<Kernel>(FULL_LDS);
+  if (e != hipSuccess) {
+    fprintf(stderr, "xfc: cannot raise the dynamic LDS limit: %s\n", hipGetErrorString(e));
+    return XFC_ERR_HIP;
+  }
+  hipLaunchKernelGGL(Kernel, g, b, (unsigned)lds, st, args);
+  return check_launch();
+}
+
+template <bool X8, int OUT>
+int launch_product(const MxPlan& p, const MxProductArgs& a, hipStream_t st) {
+  const dim3 g((unsigned)(8 * p.slots * p.tiles_m)), b(64 * MX_WAVES);
+  switch (p.nt) {
+    case 1: return launch_lds<mx4_product_kernel<1, X8, OUT>>(g, b, p.lds, st, a);
+    case 2: return launch_lds<mx4_product_kernel<2, X8, OUT>>(g, b, p.lds, st, a);
+    case 4: return launch_lds<mx4_product_kernel<4, X8, OUT>>(g, b, p.lds, st, a);
+    default: return launch_lds<mx4_product_kernel<8, X8, OUT>>(g, b, p.lds, st, a);
+  }
+}
+int launch_product(int out, bool x8, const MxPlan& p, const MxProductArgs& a, hipStream_t st) {
+  if (x8) {
+    if (out == MX_LOGITS) return launch_product<true, MX_LOGITS>(p, a, st);
+    if (out == MX_LOGITS_MAX) return launch_product<true, MX_LOGITS_MAX>(p, a, st);
+    return launch_product<true, MX_MAXIMA>(p, a, st);
+  }
+  if (out == MX_LOGITS) return launch_product<false, MX_LOGITS>(p, a, st);
+  if (out == MX_LOGITS_MAX) return launch_product<false, MX_LOGITS_MAX>(p, a, st);
+  return launch_product<false, MX_MAXIMA>(p, a, st);
+}
+
+// Rows of one launch: the row tiles of an XCD's workgroups.
+constexpr int64_t MX_ROWS = 2048;
+
+// All rows of a product, in as many launches as it takes.
+int mx_product(int out, bool x8, const void* X, int type, int64_t ldx, const void* codes, const void* scales, half_t* logits, int64_t ldo,
+               half_t* hmax, float* bmax, int64_t ldb, int64_t B, int64_t L, int64_t d, int run, hipStream_t st) {
+  for (int64_t r0 = 0; r0 < B; r0 += MX_ROWS) {
+    const int64_t rows = B - r0 < MX_ROWS ? B - r0 : MX_ROWS;
+    const MxPlan p = mx_plan(rows, L, d, x8, run, num_cus());
+    if (p.nt == 0) return XFC_ERR_LIMIT;
+    MxProductArgs a = {};
+    a.X = reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type); a.type = type; a.ldx = ldx;
+    a.codes = (const uint8_t*)codes; a.scales = (const uint8_t*)scales;
+    a.out = logits ? logits + r0 * ldo : nullptr; a.ldo = ldo;
+    a.hmax = hmax ? hmax + r0 * ldb : nullptr; a.bmax = bmax ? bmax + r0 * ldb : nullptr; a.ldb = ldb;
+    a.M = (int)rows; a.N = (int)L; a.K = (int)d;
+    a.units = ceil_div(L, MX_UNIT); a.blocks = mx_blocks(d); a.steps = mx_steps(d);
+    a.tiles_m = p.tiles_m; a.slots = p.slots; a.run = run;
+    const int rc = launch_product(out, x8, p, a, st);
+    if (rc) return rc;
+  }
+  return XFC_OK;
+}
+
+int check_product(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d, int bits) {
+  if (!dims_ok(B) || !dims_ok(L) || !dims_ok(d) || !type_ok(type) || (bits != 4 && bits != 8)) return XFC_ERR_INVALID;
+  if (B == 0 || L == 0) return XFC_OK;
+  if (!X || !codes || !scales || d <= 0) return XFC_ERR_INVALID;
+  if (d % 8 || !rows_ok(X, type, ldx) || !aligned16(codes) || !aligned16(scales)) return XFC_ERR_ALIGN;
+  if (ldx < d) return XFC_ERR_SHAPE;
+  if (mx_lds_of(1, bits == 8, d) > FULL_LDS || L > TOPK_RANGE_MAX) return XFC_ERR_LIMIT;
+  return XFC_OK;
+}
+
+int64_t mx_max_blocks(int64_t L) { return round_up(2 * (int64_t)ceil_div(L, MX_UNIT), 8); }  // maxima of a row, whole runs
+
+}  // namespace
+
+int xfc::init_labels() {
+  hipError_t e = hipSuccess;
+  auto keep = [&](hipError_t r) { if (e == hipSuccess) e = r; };
+  auto products = [&](auto x8, auto out) {
+    constexpr bool X8 = decltype(x8)::value;
+    constexpr int OUT = decltype(out)::value;
+    keep(raise_lds_limit<mx4_product_kernel<1, X8, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_product_kernel<2, X8, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_product_kernel<4, X8, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_product_kernel<8, X8, OUT>>(FULL_LDS));
+  };
+  auto both = [&](auto out) { products(std::true_type{}, out); products(std::false_type{}, out); };
+  both(std::integral_constant<int, MX_LOGITS>{});
+  both(std::integral_constant<int, MX_LOGITS_MAX>{});
+  both(std::integral_constant<int, MX_MAXIMA>{});
+  return e == hipSuccess ? XFC_OK : XFC_ERR_HIP;
+}
+
+extern "C" {
+
+size_t xfc_mx4_code_bytes(int64_t L, int64_t d) {
+  if (!dims_ok(L) || !dims_ok(d)) return 0;
+  return (size_t)ceil_div(L, MX_UNIT) * (size_t)mx_code_bytes(d);
+}
+size_t xfc_mx4_scale_bytes(int64_t L, int64_t d) {
+  if (!dims_ok(L) || !dims_ok(d)) return 0;
+  return (size_t)ceil_div(L, MX_UNIT) * (size_t)mx_scale_bytes(d);
+}
+
+int xfc_mx4_quantize(const void* W, int type, int64_t ldw, int64_t L, int64_t d, void* codes, void* scales, void* stream) {
+  bool empty;
+  const int rc = check_mx(W, type, ldw, L, d, codes, scales, empty);
+  if (rc || empty) return rc;
+  const MxArgs a = {W, nullptr, ldw, (uint8_t*)codes, (uint8_t*)scales, L, (int)d, mx_blocks(d), mx_steps(d)};
+  const dim3 g((unsigned)(ceil_div(L, MX_UNIT) * (int64_t)a.steps));
+  return by_type(type, [&](auto t) { return launch_k<mx4_quantize_kernel<decltype(t)::value>>(g, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a); });
+}
+
+int xfc_mx4_dequantize(const void* codes, const void* scales, int64_t L, int64_t d, void* W, int type, int64_t ldw, void* stream) {
+  bool empty;
+  const int rc = check_mx(W, type, ldw, L, d, codes, scales, empty);
+  if (rc || empty) return rc;
+  const MxArgs a = {nullptr, W, ldw, (uint8_t*)const_cast<void*>(codes), (uint8_t*)const_cast<void*>(scales), L, (int)d, mx_blocks(d), mx_steps(d)};
+  const dim3 g((unsigned)(ceil_div(L, MX_UNIT) * (int64_t)a.steps));
+  return by_type(type, [&](auto t) { return launch_k<mx4_dequantize_kernel<decltype(t)::value>>(g, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a); });
+}
+
+int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, const void* scales, void* out, int64_t ldo,
+                   int64_t B, int64_t L, int64_t d, int embed_bits, void* stream) {
+  const int rc = check_product(X, type, ldx, codes, scales, B, L, d, embed_bits);
+  if (rc || B == 0 || L == 0) return rc;
+  if (!out) return XFC_ERR_INVALID;
+  if (ldo % 8 || !aligned16(out)) return XFC_ERR_ALIGN;
+  if (ldo < L) return XFC_ERR_SHAPE;
+  return mx_product(MX_LOGITS, embed_bits == 8, X, type, ldx, codes, scales, (half_t*)out, ldo, nullptr, nullptr, 0, B, L, d, 1,
+                    reinterpret_cast<hipStream_t>(stream));
+}
+
+// K > 8: the logits of this many rows, and the maxima of their blocks
+static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
+  const size_t logits = (size_t)rows * (size_t)round_up(L, 8) * 2;
+  return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_max_blocks(L) * 2 : 0);
+}
+
+size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K) {
+  if (!dims_ok(B) || !dims_ok(L) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
+  if (K <= TOPK_MAX) return (size_t)B * (size_t)mx_max_blocks(L) * 4;
+  return mx_logit_rows_bytes(B, L, K);
+}
+
+int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,
+                 int64_t numy, int K, int embed_bits, float* values, int64_t* indices, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_product(X, type, ldx, codes, scales, B, L, d, embed_bits);
+  if (rc || B == 0) return rc;
+  if (K < 1 || K > SEL_MAX_K || L < K || numy < 1 || !values || !indices) return XFC_ERR_INVALID;
+  const int64_t least = B < 256 || K <= TOPK_MAX ? B : 256;
+  if (!workspace || workspace_bytes < xfc_mx4_topk_workspace_bytes(least, L, K)) return XFC_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return XFC_ERR_ALIGN;
+  const bool x8 = embed_bits == 8;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int64_t ldb = mx_max_blocks(L);
+  if (K > TOPK_MAX) {
+    int64_t block = B;
+    if (workspace_bytes < xfc_mx4_topk_workspace_bytes(B, L, K)) block = (int64_t)(workspace_bytes / xfc_mx4_topk_workspace_bytes(256, L, K)) * 256;
+    const int64_t ldl = round_up(L, 8);
+    for (int64_t r0 = 0; r0 < B; r0 += block) {
+      const int64_t rows = B - r0 < block ? B - r0 : block;
+      half_t* const logits = (half_t*)workspace;
+      half_t* const hmax = select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? logits + round_up(rows * ldl, 8) : nullptr;
+      rc = mx_product(hmax ? MX_LOGITS_MAX : MX_LOGITS, x8, reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type), type, ldx, codes, scales,
+                      logits, ldl, hmax, nullptr, ldb, rows, L, d, 1, st);
+      if (rc) return rc;
+      rc = select_rows(logits, ldl, (int)rows, (int)L, numy, K, hmax, ldb, values + r0 * K, indices + r0 * K, st);
+      if (rc) return rc;
+    }
+    return XFC_OK;
+  }
+  float* const bmax = (float*)workspace;
+  rc = mx_product(MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d, 1, st);
+  if (rc) return rc;
+  PickArgs k = {};
+  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, 32); k.N = (int)L; k.K = (int)d; k.topk = K;
+  k.begin = k.end = 1; k.numy = numy; k.out_v = values; k.out_i = indices;
+  auto pick = [&](auto s) {
+    using S = decltype(s);
+    hipLaunchKernelGGL((topk_pick_kernel<32, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 18 KB at most
+    return check_launch();
+  };
+  if (x8) return pick(MxScores<true>{X, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales});
+  return pick(MxScores<false>{X, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales});
+}
+
+// Enough workgroups to fill the chip where the rows alone do not, of a wave's 64 pairs or more each.
+static int pref_splits(int64_t B, int64_t P) {
+  const int64_t pairs = ceil_div(P, B);
+  int64_t s = ceil_div(1024, B);
+  const int64_t most = ceil_div(pairs, PREF_WAVES * pref_pairs(1));
+  if (s > most) s = most;
+  return s < 1 ? 1 : (int)s;
+}
+size_t xfc_preference_workspace_bytes(int64_t B, int64_t P, int64_t d) {
+  if (!dims_ok(B) || !dims_ok(P) || !dims_ok(d) || B == 0) return 16;
+  const int64_t s = pref_splits(B, P);
+  return (size_t)round_up(B * s * 8, 16) + (size_t)round_up(P * 4, 16) + (s > 1 ? (size_t)(B * s * d * 4) : 0);
+}
+
+int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t ldw, const void* scales, int64_t L, int64_t d,
+                   const int32_t* rowptr, const int32_t* chosen, const int32_t* rejected, const float* reference, const float* weight,
+                   int64_t B, int64_t P, float beta, float smoothing, float scale, float* loss, float* margin,
+                   void* dX, int dx_type, int64_t lddx, void* G, int64_t ldg, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!dims_ok(B) || !dims_ok(L) || !dims_ok(d) || !dims_ok(P) || !type_ok(type) || (dX && !type_ok(dx_type))) return XFC_ERR_INVALID;
+  if (!loss || (B > 0 && (!X || !W || !rowptr)) || (P > 0 && (!chosen || !rejected)) || d <= 0 || L <= 0 || B > 0x7fffff) return XFC_ERR_INVALID;
+  if (!(beta == beta) || !(smoothing >= 0.f && smoothing <= 1.f)) return XFC_ERR_INVALID;
+  if (B > 0 && (d % 8 || !rows_ok(X, type, ldx) || !aligned16(W) || (scales ? !aligned16(scales) : ldw % 8 != 0))) return XFC_ERR_ALIGN;
+  if (B > 0 && (ldx < d || (!scales && ldw < d) || (dX && lddx < d) || (G && ldg < L))) return XFC_ERR_SHAPE;
+  if (d > 4096) return XFC_ERR_LIMIT;
+  if (!workspace || workspace_bytes < xfc_preference_workspace_bytes(B, P, d)) return XFC_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return XFC_ERR_ALIGN;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  PrefArgs a = {};
+  a.X = X; a.type = type; a.ldx = ldx; a.W = W; a.ldw = ldw; a.scales = (const uint8_t*)scales; a.L = L; a.d = (int)d;
+  a.rowptr = rowptr; a.chosen = chosen; a.rejected = rejected; a.reference = reference; a.weight = weight;
+  a.B = (int)B; a.P = (int)P; a.splits = B > 0 ? pref_splits(B, P) : 1;
+  a.beta = beta; a.smoothing = smoothing; a.scale = scale; a.margin = margin;
+  a.dX = dX; a.dx_type = dx_type; a.lddx = lddx; a.G = (half_t*)G; a.ldg = ldg; a.loss = loss;
+  a.part_loss = (double*)workspace;
+  a.slope = (float*)((char*)workspace + round_up((int64_t)a.B * a.splits * 8, 16));
+  a.part_dx = (float*)((char*)a.slope + round_up(P * 4, 16));
+  if (B > 0) {
+    const dim3 g((unsigned)B, (unsigned)a.splits), b(64 * PREF_WAVES);
+    auto launch = [&](auto c) {
+      constexpr int C = decltype(c)::value;
+      return scales ? launch_k<preference_kernel<C, true>>(g, b, 0, st, a) : launch_k<preference_kernel<C, false>>(g, b, 0, st, a);
+    };
+    const int rc = d <= 512 ? launch(std::integral_constant<int, 1>{}) : d <= 1024 ? launch(std::integral_constant<int, 2>{})
+                 : d <= 2048 ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 8>{});
+    if (rc) return rc;
+  }
+  const bool rows = B > 0 && (G || (dX && a.splits > 1));
+  return launch_k<preference_finish_kernel>(dim3((unsigned)(rows ? B + 1 : 1)), dim3(256), 0, st, a);
+}
+
+}  // extern "C"

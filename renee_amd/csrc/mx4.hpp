@@ -1,0 +1,514 @@
+// Label matrices in microscaled 4-bit floating point (MX4): quantisation, and products of embeddings with them.
+//
+// 32 consecutive dims of a label are a block: a scale 2^(byte - 127) and 32 numbers of a sign, two exponent bits and one mantissa
+// bit (0, 0.5, 1, 1.5, 2, 3, 4, 6).  byte - 127 = floor(log2 of the block's largest magnitude) - 2, at least -127, so that the largest
+// number is 4 or 6; numbers are rounded to the nearest, ties to an even mantissa, and those above 6 become 6.  A block that
+// holds an infinity or a NaN has byte 255 and stands for 32 NaNs; a block of zeros has byte 0.
+//
+// Embeddings enter a product in blocks of the same kind, quantised as they are loaded: in 4 bits, or in 8 (four exponent
+// bits, three mantissa bits, up to 448: byte - 127 = floor(log2 of the largest) - 8).  Then z[b][l] = sum over blocks of 2^(sx + sw) times
+// the sum of 32 products, which is what v_mfma_scale_f32_16x16x128_f8f6f4 does: 16 rows x 16 labels x four blocks, sums in fp32.
+// With 4-bit embeddings products are quarters and sums are exact unless scales lie some 2^8 apart.  With 8-bit ones the
+// matrix pipe drops what lies below about 2^-14 of the largest of neighbouring products (measured), well under fp16's half step.
+//
+// Layout.  Lane (i, q) = i + 16 q of the MFMA holds row i, block q of the step.  Labels go in units of 64, four tiles of 16 for one
+// wave, dims in steps of four blocks, and codes and scales lie in the order in which lanes take them:
+//   codes   [unit][step][tile 4][row 16][block 4][16 bytes]    the last step has as many blocks as are left of the width
+//   scales  [unit][step][block 4][row 16][tile 4]              a lane's dword: one byte for each tile, the MFMA's operand selector
+// so that a fetch of a wave is 1 KB in a row, 24 KB of a unit at 768 dims follow each other, and a scale takes no instruction but its load.
+// Row 4 q + r of tile 2 p + t is label 32 p + 8 q + 4 t + r of the unit: of two tiles' sums a lane then holds eight consecutive labels.
+#pragma once
+#include <type_traits>
+#include <utility>
+
+#include "pipe_core.hpp"
+#include "topk.hpp"
+
+namespace xfc {
+
+constexpr int MX_BLOCK = 32, MX_UNIT = 64, MX_STEP = 128;  // dims of a block, labels of a unit, dims of a step
+constexpr int MX_TILES = MX_UNIT / 16;
+constexpr uint32_t MX_NAN = 255;
+
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef int int8v __attribute__((ext_vector_type(8)));
+
+__host__ __device__ inline int mx_blocks(int64_t d) { return (int)((d + MX_BLOCK - 1) / MX_BLOCK); }
+__host__ __device__ inline int mx_steps(int64_t d) { return (int)((d + MX_STEP - 1) / MX_STEP); }
+// bytes of a unit
+__host__ __device__ inline int64_t mx_code_bytes(int64_t d) { return (int64_t)MX_UNIT * MX_BLOCK / 2 * mx_blocks(d); }
+__host__ __device__ inline int64_t mx_scale_bytes(int64_t d) { return (int64_t)MX_UNIT * 4 * mx_steps(d); }
+
+// The label of a unit that row i of tile t is, and back.
+__host__ __device__ inline int mx_label(int t, int i) { return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3); }
+__host__ __device__ inline int mx_tile(int label) { return 2 * (label >> 5) + ((label >> 2) & 1); }
+__host__ __device__ inline int mx_row(int label) { return 4 * ((label >> 3) & 3) + (label & 3); }
+
+// Where in its unit a label's block stands: codes (16 bytes), scale.
+__host__ __device__ inline int mx_code_at(int tile, int row, int block, int blocks) {
+  const int step = block >> 2, wide = blocks - 4 * step < 4 ? blocks - 4 * step : 4;
+  return step * 4096 + ((tile * 16 + row) * wide + (block & 3)) * 16;
+}
+__host__ __device__ inline int mx_scale_at(int tile, int row, int block) { return (block >> 2) * 256 + (block & 3) * 64 + row * 4 + tile; }
+
+// ---------------------------------------------------------------------------------------------
+// blocks
+// ---------------------------------------------------------------------------------------------
+struct Float8 { float v[8]; };
+
+// Eight consecutive numbers of type TYPE (xfc_type), as floats.
+template <int TYPE>
+__device__ __forceinline__ Float8 load8(const void* p) {
+  Float8 f;
+  if constexpr (TYPE == XFC_F32) {
+    const float4v lo = reinterpret_cast<const float4v*>(p)[0], hi = reinterpret_cast<const float4v*>(p)[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { f.v[e] = lo[e]; f.v[4 + e] = hi[e]; }
+  } else if constexpr (TYPE == XFC_BF16) {
+    const uint4v q = *reinterpret_cast<const uint4v*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { f.v[2 * e] = __uint_as_float(q[e] << 16); f.v[2 * e + 1] = __uint_as_float(q[e] & 0xffff0000u); }
+  } else {
+    const half8 h = *reinterpret_cast<const half8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = (float)h[e];
+  }
+  return f;
+}
+constexpr int type_bytes(int type) { return type == XFC_F32 ? 4 : 2; }
+
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {  // over four neighbouring lanes
+  const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true);  // quad_perm 1, 0, 3, 2
+  v = a > v ? a : v;
+  const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true);  // quad_perm 2, 3, 0, 1
+  return b > v ? b : v;
+}
+
+// The scale byte of a block that lies in four neighbouring lanes, eight numbers each, and the factor that conversions divide by.
+// Magnitudes are compared as bits: infinities and NaNs come out on top.  Where the scale would be no normal float, numbers and
+// factor are multiplied by 2^64, which leaves the quotient as it is.
+template <int EMAX>
+__device__ __forceinline__ uint32_t block_scale(Float8& f, float& by) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __float_as_uint(f.v[e]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  m = quad_max(m);
+  const int exponent = (int)(m >> 23);
+  uint32_t byte = exponent > EMAX ? exponent - EMAX : 0;
+  by = __uint_as_float(byte << 23);
+  if (byte == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] *= 0x1p64f;
+    by = 0x1p-63f;
+  }
+  return exponent == 255 ? MX_NAN : m == 0 ? 0 : byte;
+}
+__device__ __forceinline__ uint32_t to_fp4(const Float8& f, float by) {  // eight numbers, the first in the lowest bits
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f.v[0], f.v[1], by, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f.v[2], f.v[3], by, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f.v[4], f.v[5], by, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f.v[6], f.v[7], by, 3);
+}
+// (The conversion makes a NaN of what lies above 448: that is cut off first.)
+__device__ __forceinline__ uint64_t to_fp8(Float8 f, float by) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f.v[e] = __builtin_amdgcn_fmed3f(f.v[e], -448.f * by, 448.f * by);
+  typedef short short2v __attribute__((ext_vector_type(2)));
+  short2v lo = {0, 0}, hi = {0, 0};
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, f.v[0], f.v[1], by, false);
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, f.v[2], f.v[3], by, true);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, f.v[4], f.v[5], by, false);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, f.v[6], f.v[7], by, true);
+  return (uint64_t)__builtin_bit_cast(uint32_t, lo) | ((uint64_t)__builtin_bit_cast(uint32_t, hi) << 32);
+}
+// 2^(byte - 127), NaN for 255
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == MX_NAN ? 0x7fc00000u : byte == 0 ? 0x00400000u : byte << 23);
+}
+// Eight numbers of a block, from their codes.
+__device__ __forceinline__ Float8 from_fp4(uint32_t codes, float scale) {
+  Float8 f;
+  auto pair = [&](auto at) {
+    const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, decltype(at)::value);
+    f.v[2 * decltype(at)::value] = p[0] * scale;
+    f.v[2 * decltype(at)::value + 1] = p[1] * scale;
+  };
+  pair(std::integral_constant<int, 0>{});
+  pair(std::integral_constant<int, 1>{});
+  pair(std::integral_constant<int, 2>{});
+  pair(std::integral_constant<int, 3>{});
+  return f;
+}
+
+// ---------------------------------------------------------------------------------------------
+// label matrix -> MX4 and back
+// ---------------------------------------------------------------------------------------------
+// A workgroup takes a step of a unit: 64 labels x 128 dims.  Of each tile a wave takes four rows, four consecutive labels, a lane eight
+// dims of one: 256 bytes of a label in a row are read (fp16), 256 bytes of codes written, and after four tiles a lane in four has
+// a dword of scales.  Bound by the stream.
+struct MxArgs {
+  const void* W; void* out; int64_t ldw;  // quantize: W, dequantize: out
+  uint8_t* codes; uint8_t* scales;
+  int64_t L; int d, blocks, steps;
+};
+
+template <int TYPE>
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(MxArgs a) {
+  const int64_t unit = blockIdx.x / (unsigned)a.steps;
+  const int step = blockIdx.x % (unsigned)a.steps;
+  const int lane = threadIdx.x & 63, row = 4 * (threadIdx.x >> 6) + (lane >> 4), block = (lane >> 2) & 3, part = lane & 3;
+  const int k = step * MX_STEP + block * MX_BLOCK + part * 8;
+  const int wide = a.blocks - 4 * step < 4 ? a.blocks - 4 * step : 4;
+  Float8 f[MX_TILES];
+#pragma unroll
+  for (int t = 0; t < MX_TILES; ++t) {
+    const int64_t label = unit * MX_UNIT + mx_label(t, row);
+    f[t] = Float8{};
+    if (label < a.L && k < a.d) f[t] = load8<TYPE>(reinterpret_cast<const char*>(a.W) + (label * a.ldw + k) * type_bytes(TYPE));
+  }
+  uint32_t bytes = 0;
+  uint8_t* const codes = a.codes + unit * mx_code_bytes(a.d) + step * 4096;
+#pragma unroll
+  for (int t = 0; t < MX_TILES; ++t) {
+    float by;
+    const uint32_t byte = block_scale<2>(f[t], by);
+    bytes |= byte << (8 * t);
+    if (block < wide) *reinterpret_cast<uint32_t*>(codes + ((t * 16 + row) * wide + block) * 16 + part * 4) = to_fp4(f[t], by);
+  }
+  if (part == 0) *reinterpret_cast<uint32_t*>(a.scales + unit * mx_scale_bytes(a.d) + step * 256 + block * 64 + row * 4) = bytes;
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(256) mx4_dequantize_kernel(MxArgs a) {
+  const int64_t unit = blockIdx.x / (unsigned)a.steps;
+  const int step = blockIdx.x % (unsigned)a.steps;
+  const int lane = threadIdx.x & 63, row = 4 * (threadIdx.x >> 6) + (lane >> 4), block = (lane >> 2) & 3, part = lane & 3;
+  const int k = step * MX_STEP + block * MX_BLOCK + part * 8;
+  const int wide = a.blocks - 4 * step < 4 ? a.blocks - 4 * step : 4;
+  if (block >= wide || k >= a.d) return;
+  const uint32_t bytes = *reinterpret_cast<const uint32_t*>(a.scales + unit * mx_scale_bytes(a.d) + step * 256 + block * 64 + row * 4);
+  const uint8_t* const codes = a.codes + unit * mx_code_bytes(a.d) + step * 4096;
+#pragma unroll
+  for (int t = 0; t < MX_TILES; ++t) {
+    const int64_t label = unit * MX_UNIT + mx_label(t, row);
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + ((t * 16 + row) * wide + block) * 16 + part * 4);
+    const Float8 f = from_fp4(c, scale_value((bytes >> (8 * t)) & 255u));
+    if (label >= a.L) continue;
+    char* const to = reinterpret_cast<char*>(a.out) + (label * a.ldw + k) * type_bytes(TYPE);
+    if constexpr (TYPE == XFC_F32) {
+      reinterpret_cast<float4v*>(to)[0] = float4v{f.v[0], f.v[1], f.v[2], f.v[3]};
+      reinterpret_cast<float4v*>(to)[1] = float4v{f.v[4], f.v[5], f.v[6], f.v[7]};
+    } else if constexpr (TYPE == XFC_BF16) {
+      typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+      bf16x8 h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = (__bf16)f.v[e];
+      *reinterpret_cast<bf16x8*>(to) = h;
+    } else {
+      half8 h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = (half_t)f.v[e];
+      *reinterpret_cast<half8*>(to) = h;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// embeddings in blocks, as the B side of the product
+// ---------------------------------------------------------------------------------------------
+// A fragment is 16 rows x one step: 1 KB of codes in 4 bits, 2 KB in 8, lane after lane.  In 8 bits the MFMA takes dims 16 q .. 16 q
+// + 15 of the step from lane (i, q)'s first sixteen bytes and 64 + 16 q .. from the other sixteen (checked on hardware), so that block b is
+// half b / 2 of lanes (i, 2 (b % 2)) and (i, 2 (b % 2) + 1); its scale is lane (i, b)'s all the same.
+template <bool X8>
+struct MxRows {
+  static constexpr int FRAG = X8 ? 2048 : 1024;
+  static constexpr int EMAX = X8 ? 8 : 2;
+  // Where the eight numbers `part` of row i's block stand.
+  static __device__ __forceinline__ int at(int i, int block, int part) {
+    if constexpr (X8) return (block >> 1) * 1024 + ((2 * (block & 1) + (part >> 1)) * 16 + i) * 16 + (part & 1) * 8;
+    else return (block * 16 + i) * 16 + part * 4;
+  }
+  // Quantises them (four neighbouring lanes hold a block) and returns the scale byte.
+  static __device__ __forceinline__ uint32_t put(unsigned char* frag, Float8 f, int i, int block, int part) {
+    float by;
+    const uint32_t byte = block_scale<EMAX>(f, by);
+    if constexpr (X8) *reinterpret_cast<uint64_t*>(frag + at(i, block, part)) = to_fp8(f, by);
+    else *reinterpret_cast<uint32_t*>(frag + at(i, block, part)) = to_fp4(f, by);
+    return byte;
+  }
+  static __device__ __forceinline__ int8v get(const unsigned char* frag, int lane) {
+    const int4v lo = *reinterpret_cast<const int4v*>(frag + lane * 16);
+    if constexpr (X8) {
+      const int4v hi = *reinterpret_cast<const int4v*>(frag + 1024 + lane * 16);
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return __builtin_shufflevector(lo, lo, 0, 1, 2, 3, -1, -1, -1, -1);
+  }
+};
+
+// c + labels (codes a, scale byte T of sa) . rows (codes b, scale byte J of sb)
+template <bool X8, int T, int J>
+__device__ __forceinline__ float4v mx_mfma(const int4v& a, uint32_t sa, const int8v& b, uint32_t sb, const float4v& c) {
+  const int8v a8 = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b, c, 4, X8 ? 0 : 4, T, (int)sa, J, (int)sb);
+}
+
+// Eight numbers of a row of an embedding matrix of any type.
+__device__ __forceinline__ Float8 load8_of(const void* X, int type, int64_t at) {
+  if (type == XFC_F32) return load8<XFC_F32>(reinterpret_cast<const float*>(X) + at);
+  if (type == XFC_BF16) return load8<XFC_BF16>(reinterpret_cast<const uint16_t*>(X) + at);
+  return load8<XFC_F16>(reinterpret_cast<const half_t*>(X) + at);
+}
+
+// ---------------------------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------------------------
+enum MxOut { MX_LOGITS, MX_LOGITS_MAX, MX_MAXIMA };
+
+struct MxProductArgs {
+  const void* X; int type; int64_t ldx;  // M rows of K
+  const uint8_t* codes; const uint8_t* scales;
+  half_t* out; int64_t ldo;              // logits
+  half_t* hmax; float* bmax; int64_t ldb; // maxima of blocks of 32 labels: of the logits as stored, of the sums
+  int M, N, K;
+  int units, blocks, steps;
+  int tiles_m, slots;                    // row tiles; workgroups of a row tile on an XCD
+  int run;                               // units in a row that a wave takes, 1 or 4
+};
+
+constexpr int MX_WAVES = 8, MX_SLOTS = 3;
+
+// rows of a workgroup: NT tiles of 16
+template <int NT, bool X8>
+constexpr int64_t mx_lds(int64_t d) { return (int64_t)mx_steps(d) * (NT * MxRows<X8>::FRAG + (NT + 3) / 4 * 256); }
+
+// A workgroup keeps its rows' fragments in the LDS and its waves, which never meet again, stream units of 64 labels past them, straight
+// into the A side's registers: MX_SLOTS - 1 steps on their way, across units.
+template <int NT, bool X8, int OUT>
+__global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_kernel(MxProductArgs a) {
+  using Rows = MxRows<X8>;
+  constexpr int NS = (NT + 3) / 4;  // dwords of row scales of a step
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
+  unsigned char* const frags = smem_raw;
+  unsigned char* const row_scales = smem_raw + a.steps * NT * Rows::FRAG;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+  const int row0 = (local % a.tiles_m) * 16 * NT;
+  const int workers = 8 * a.slots * MX_WAVES, worker = (xcd * a.slots + local / a.tiles_m) * MX_WAVES + wave;
+  const int run = a.run, skip = (workers - 1) * run + 1;  // from the last unit of a run to the first of the next
+  auto next = [&](int u) { return (u + 1) & (run - 1) ? u + 1 : u + skip; };
+  int unit = worker * run;
+
+  // Fetch cursor.  Past the last unit it repeats that one, so that as many loads are on their way as ever.
+  const int64_t unit_codes = mx_code_bytes(a.K), unit_scales = mx_scale_bytes(a.K);
+  const int whole = a.blocks >> 2, wide = a.blocks & 3;  // steps of four blocks, blocks of the step behind them
+  const uint32_t at_whole = (uint32_t)(4 * i + q) * 16, at_rest = (uint32_t)(wide * i + (q < wide ? q : wide - 1)) * 16;
+  int f_unit = unit < a.units ? unit : a.units - 1, f_step = 0;
+  struct Slot { int4v w[MX_TILES]; uint32_t s; };
+  Slot slot[MX_SLOTS];
+  auto fetch = [&](Slot& to) {
+    const uint8_t* const c = a.codes + (int64_t)f_unit * unit_codes + f_step * 4096;
+    const uint8_t* const s = a.scales + (int64_t)f_unit * unit_scales + f_step * 256;
+    const bool rest = f_step == whole;
+    const uint32_t at = rest ? at_rest : at_whole, tile = rest ? (uint32_t)wide * 256 : 1024u;
+#pragma unroll
+    for (int t = 0; t < MX_TILES; ++t) to.w[t] = *reinterpret_cast<const int4v*>(c + t * tile + at);
+    to.s = *reinterpret_cast<const uint32_t*>(s + (uint32_t)lane * 4);
+    if (++f_step == a.steps) {
+      f_step = 0;
+      if (next(f_unit) < a.units) f_unit = next(f_unit);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < MX_SLOTS; ++s) fetch(slot[s]);
+
+  // The rows' blocks, four lanes each, 16 lanes a step of a row; behind the last row, dim or block there are zeros.
+  for (int w = tid; w < a.steps * NT * 256; w += 64 * MX_WAVES) {
+    const int part = w & 3, block = (w >> 2) & 3, step = (w >> 4) % a.steps, r = (w >> 4) / a.steps;
+    const int k = step * MX_STEP + block * MX_BLOCK + part * 8;
+    Float8 f = {};
+    if (row0 + r < a.M && k < a.K) f = load8_of(a.X, a.type, (int64_t)(row0 + r) * a.ldx + k);
+    const int j = r >> 4;
+    const uint32_t byte = Rows::put(frags + (step * NT + j) * Rows::FRAG, f, r & 15, block, part);
+    if (part == 0) row_scales[((step * NS + (j >> 2)) * 64 + block * 16 + (r & 15)) * 4 + (j & 3)] = (unsigned char)byte;
+  }
+  __syncthreads();
+
+  float4v acc[MX_TILES][NT];
+  [[maybe_unused]] float best[(NT + 1) / 2][4];
+  int step = 0;
+
+  auto multiply = [&](const Slot& w, auto first) {
+    uint32_t sb[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) sb[n] = *reinterpret_cast<const uint32_t*>(row_scales + ((step * NS + n) * 64 + lane) * 4);
+    auto row_tile = [&](auto jt) {
+      constexpr int J = decltype(jt)::value;
+      const int8v b = Rows::get(frags + (step * NT + J) * Rows::FRAG, lane);
+      auto tile = [&](auto tt) {
+        constexpr int T = decltype(tt)::value;
+        acc[T][J] = mx_mfma<X8, T, J % 4>(w.w[T], w.s, b, sb[J / 4], decltype(first)::value ? float4v{0.f, 0.f, 0.f, 0.f} : acc[T][J]);
+      };
+      [&]<int... T>(std::integer_sequence<int, T...>) { (tile(std::integral_constant<int, T>{}), ...); }(std::make_integer_sequence<int, MX_TILES>{});
+    };
+    [&]<int... J>(std::integer_sequence<int, J...>) { (row_tile(std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, NT>{});
+  };
+
+  auto epilogue = [&]() {
+    const int label0 = unit * MX_UNIT;
+    const bool edge = label0 + MX_UNIT > a.N;
+    if constexpr (OUT == MX_MAXIMA) {
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < MX_TILES; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool in = label0 + mx_label(t, 4 * q + r) < a.N;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[t][j][r] = in ? acc[t][j][r] : __builtin_nanf("");
+          }
+      }
+      auto largest = [&](int p, int j) {  // of this lane's eight labels
+        const float4v lo = acc[2 * p][j], hi = acc[2 * p + 1][j];
+        return fmaxf(fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])), fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])));
+      };
+      const int r4 = unit & (run - 1);
+#pragma unroll
+      for (int j2 = 0; j2 < (NT + 1) / 2; ++j2) {
+        // lane group g ends up with block g / 2 of row tile 2 j2 + g % 2
+        const int j1 = 2 * j2 + 1 < NT ? 2 * j2 + 1 : 2 * j2;
+        const float m = fold16(fold32(largest(0, 2 * j2), largest(1, 2 * j2)), fold32(largest(0, j1), largest(1, j1)));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) best[j2][r] = r4 == r ? m : best[j2][r];
+      }
+      const int after = next(unit);
+      if (after != unit + 1 || run == 1 || after >= a.units) {
+        const int64_t first = 2 * (int64_t)(unit - r4);
+#pragma unroll
+        for (int j2 = 0; j2 < (NT + 1) / 2; ++j2) {
+          const int row = row0 + 32 * j2 + 16 * (q & 1) + i;
+          if (2 * j2 + (q & 1) >= NT || row >= a.M) continue;
+          float* const to = a.bmax + (int64_t)row * a.ldb + first;
+          if (run == 1) to[q >> 1] = best[j2][0];
+          else
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[2 * r + (q >> 1)] = best[j2][r];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int row = row0 + 16 * j + i;
+        uint32_t largest[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          half8 h;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) { h[r] = (half_t)acc[2 * p][j][r]; h[4 + r] = (half_t)acc[2 * p + 1][j][r]; }
+          const int col = label0 + 32 * p + 8 * q;
+          if constexpr (OUT == MX_LOGITS_MAX) {
+            half8 m = h;
+            if (edge) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) m[e] = col + e < a.N ? h[e] : (half_t)-__builtin_huge_valf();
+            }
+            largest[p] = pk_max(m);
+          }
+          if (row < a.M) {
+            half_t* const to = a.out + (int64_t)row * a.ldo + col;
+            if (!edge || col + 8 <= a.N) *reinterpret_cast<half8*>(to) = h;
+            else
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (col + e < a.N) to[e] = h[e];
+          }
+        }
+        if constexpr (OUT == MX_LOGITS_MAX) {
+          const uint32_t v = pk_fold32(largest[0], largest[1]);
+          const half_t m = pk_larger(pk_fold16(v, v));
+          if (row < a.M && (q & 1) == 0) a.hmax[(int64_t)row * a.ldb + 2 * (int64_t)unit + (q >> 1)] = m;
+        }
+      }
+    }
+  };
+
+  while (unit < a.units) {
+#pragma unroll
+    for (int s = 0; s < MX_SLOTS; ++s) {
+      if (unit < a.units) {
+        if (step == 0) multiply(slot[s], std::true_type{});
+        else multiply(slot[s], std::false_type{});
+        if (++step == a.steps) {
+          epilogue();
+          step = 0;
+          unit = next(unit);
+        }
+        fetch(slot[s]);
+      }
+    }
+  }
+}
+
+// How topk_pick_kernel forms the scores of sixteen labels again: blocks of 32 labels are half units, the sixteen are one of their two
+// tiles.  The row, quantised once, stands in all sixteen columns; the MFMAs and their order are those of mx4_product_kernel.
+template <bool X8>
+struct MxScores {
+  const void* X; int type; int64_t ldx;
+  const uint8_t* codes; const uint8_t* scales;
+
+  static __device__ __forceinline__ unsigned char* room() {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
+    return smem_raw;
+  }
+  // bytes of a step: block q's numbers behind each other, then four scale bytes
+  static constexpr int STEP_BYTES = (X8 ? 128 : 64) + 16;
+  static int64_t lds(int64_t d) { return (int64_t)mx_steps(d) * STEP_BYTES; }
+
+  __device__ __forceinline__ void open(const PickArgs& a, int row) const {
+    unsigned char* const at = room();
+    for (int w = threadIdx.x; w < mx_steps(a.K) * 16; w += 512) {
+      const int part = w & 3, block = (w >> 2) & 3, step = w >> 4, k = w * 8;
+      Float8 f = {};
+      if (k < a.K) f = load8_of(X, type, (int64_t)row * ldx + k);
+      float by;
+      const uint32_t byte = block_scale<X8 ? 8 : 2>(f, by);
+      unsigned char* const s = at + step * STEP_BYTES;
+      if constexpr (X8) *reinterpret_cast<uint64_t*>(s + (block * 4 + part) * 8) = to_fp8(f, by);
+      else *reinterpret_cast<uint32_t*>(s + (block * 4 + part) * 4) = to_fp4(f, by);
+      if (part == 0) s[STEP_BYTES - 16 + block] = (unsigned char)byte;
+    }
+  }
+  static __device__ __forceinline__ int place(int part, int lane) { return 8 * (lane >> 4) + 4 * part; }
+  __device__ __forceinline__ float4v score(const PickArgs& a, int, int first, int part, int lane) const {
+    const int blocks = mx_blocks(a.K), steps = mx_steps(a.K), i = lane & 15, q = lane >> 4;
+    const int64_t unit = first / MX_UNIT;
+    const int p = (first % MX_UNIT) / 32;
+    const uint8_t* const c = codes + unit * mx_code_bytes(a.K);
+    const uint8_t* const s = scales + unit * mx_scale_bytes(a.K);
+    const unsigned char* const at = room();
+    float4v z = {0.f, 0.f, 0.f, 0.f};
+    for (int step = 0; step < steps; ++step) {
+      const int wide = blocks - 4 * step < 4 ? blocks - 4 * step : 4;
+      const int4v w = *reinterpret_cast<const int4v*>(c + mx_code_at(2 * p + part, i, 4 * step + (q < wide ? q : wide - 1), blocks));
+      const uint32_t sa = *reinterpret_cast<const uint32_t*>(s + step * 256 + lane * 4) >> (8 * (2 * p + part));
+      const unsigned char* const x = at + step * STEP_BYTES;
+      int8v b;
+      if constexpr (X8) {
+        const int4v lo = *reinterpret_cast<const int4v*>(x + q * 16), hi = *reinterpret_cast<const int4v*>(x + 64 + q * 16);
+        b = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
+        const int4v lo = *reinterpret_cast<const int4v*>(x + q * 16);
+        b = __builtin_shufflevector(lo, lo, 0, 1, 2, 3, -1, -1, -1, -1);
+      }
+      z = mx_mfma<X8, 0, 0>(w, sa, b, x[STEP_BYTES - 16 + q], z);
+    }
+    return z;
+  }
+};
+
+}  // namespace xfc

@@ -17,8 +17,17 @@
 namespace xfc {
 
 constexpr int TOPK_MAX = 8;
+constexpr int SEL_MAX_K = 8192;
+// Above TOPK_MAX (xfc_kernels.hip): the K largest of each row of fp16 logits, by the maxima of the rows' blocks of LOGIT_BLOCK where
+// bmax is given, which is of use where the first says so.
+__attribute__((visibility("hidden"))) bool select_takes_maxima(int64_t K, int64_t n_blocks);
+__attribute__((visibility("hidden"))) int select_rows(const _Float16* logits, int64_t ldl, int rows, int L, int64_t numy, int K, const _Float16* bmax,
+                                                      int64_t ldb, float* values, int64_t* indices, hipStream_t st);
 constexpr int64_t TOPK_RANGE_MAX = (int64_t)1 << 30;  // labels of a range: the kernels' 32-bit indices run somewhat past its end
 typedef float float2v __attribute__((ext_vector_type(2)));
+
+// What xfc_init does for the kernels of label_kernels.hip.
+__attribute__((visibility("hidden"))) int init_labels();
 
 // Floats as unsigned keys in the same order, and back.
 __device__ __forceinline__ uint32_t topk_key(float f) {
@@ -58,6 +67,33 @@ __device__ __forceinline__ float fold16(float a, float b) {
   asm("s_nop 1" : "+v"(a), "+v"(b));
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
   return max_num(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+constexpr int LOGIT_BLOCK = 32;
+// max of two packed halves each, and of three; an operand that is no number wins, so that a block with one can be told.
+// (Two wait states in front of the lane exchanges below, as for fold32.)
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t pk_max(const half8& v) {
+  const uint4v q = __builtin_bit_cast(uint4v, v);
+  return pk_max(pk_max(q[0], q[1], q[2]), q[3], q[3]);
+}
+__device__ __forceinline__ uint32_t pk_fold32(uint32_t a, uint32_t b) {
+  asm("s_nop 1" : "+v"(a), "+v"(b));
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  return pk_max(r[0], r[1], r[1]);
+}
+__device__ __forceinline__ uint32_t pk_fold16(uint32_t a, uint32_t b) {
+  asm("s_nop 1" : "+v"(a), "+v"(b));
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  return pk_max(r[0], r[1], r[1]);
+}
+__device__ __forceinline__ half_t pk_larger(uint32_t a) {  // of the two halves
+  const uint16_t h = (uint16_t)pk_max(a, a >> 16, a >> 16);
+  return __builtin_bit_cast(half_t, h);
 }
 
 struct ScoreArgs {
@@ -324,15 +360,51 @@ __device__ __forceinline__ unsigned long long wave_top(unsigned long long key, i
   return top;
 }
 
+// How topk_pick_kernel forms the scores of 16 labels of a block again: half weights.  open() runs once, before the first score and
+// a barrier; score() leaves four labels' scores in every lane, of which lanes 0, 16, 32 and 48 are kept, at place() in the block.
+struct HalfScores {
+  static constexpr int STEPS = 8;  // pieces of the weights on their way
+  __device__ __forceinline__ void open(const PickArgs&, int) const {}
+  static __device__ __forceinline__ int place(int part, int lane) { return part * 16 + 4 * (lane >> 4); }
+  __device__ __forceinline__ float4v score(const PickArgs& a, int row, int first, int part, int lane) const {
+    const int label = first + part * 16, mine_l = label + (lane & 15), k8 = 8 * (lane >> 4);
+    const half_t* wp = a.W + (int64_t)(mine_l < a.N ? mine_l : a.N - 1) * a.ldw;
+    const half_t* xp = a.X + (int64_t)row * a.ldx;
+    float4v z = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < a.K; k0 += 32 * STEPS) {
+      half8 wv[STEPS], xv[STEPS];
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        const int k = k0 + 32 * j + k8;
+        wv[j] = *reinterpret_cast<const half8*>(wp + (k < a.K ? k : 0));
+        xv[j] = *reinterpret_cast<const half8*>(xp + (k < a.K ? k : 0));
+      }
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        if (k0 + 32 * j >= a.K) break;
+        if (k0 + 32 * j + 32 > a.K) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            wv[j][e] = k0 + 32 * j + k8 < a.K ? wv[j][e] : (half_t)0.f;
+            xv[j][e] = k0 + 32 * j + k8 < a.K ? xv[j][e] : (half_t)0.f;
+          }
+        }
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv[j], xv[j], z, 0, 0, 0);
+      }
+    }
+    return z;
+  }
+};
+
 // One workgroup per row.  With few blocks or many rows bound by its instructions (25 us at 700 rows x 282 blocks, where seven of
 // a thread's eight fetches brought nothing and six of the eight waves put zeros in order): what has nothing to do is left out.  Else by reading the blocks' maxima and the chosen blocks' weights (1024 rows x 87,885 blocks, K = 5: 122 us,
 // 5 TB/s), on small batches by latency (16 x 8,192 blocks: 14 us): each thread finds the best of its blocks,
 // the K best threads are looked at again block by block (a wave each), and the K best blocks' scores are formed by MFMAs
 // that hold the row in all sixteen columns.  Keys are (score, id) as topk_entry makes them, all different but for 0.
-template <int BLOCK>
-__global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a) {
+template <int BLOCK, class Scores = HalfScores>
+__global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a, Scores scores) {
   constexpr int NW = 8, LISTS = NW * TOPK_MAX;
-  constexpr int FETCH = 8, STEPS = 8;  // loads on their way: maxima, pieces of the weights
+  constexpr int FETCH = 8;  // maxima on their way
   static_assert(TOPK_MAX * BLOCK <= 512 - TOPK_MAX, "one candidate per thread");
   __shared__ unsigned long long list[LISTS], chosen[TOPK_MAX], kept[TOPK_MAX];
   __shared__ float score[TOPK_MAX * BLOCK];
@@ -365,6 +437,7 @@ __global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a) {
     __syncthreads();
   };
 
+  scores.open(a, row);
   if (tid < TOPK_MAX) kept[tid] = a.best && !a.begin && tid < K ? a.best[(int64_t)row * K + tid] : 0ull;
   unsigned long long bound = ~0ull;  // blocks at or above it have been taken
   for (;;) {
@@ -413,33 +486,9 @@ __global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a) {
     n_sel = __builtin_amdgcn_readfirstlane(n_sel);
     // their scores, 16 labels at a time; the MFMAs and their order are those of the kernels above
     for (int u = wave; u < n_sel * (BLOCK / 16); u += NW) {
-      const int label = (int)~(uint32_t)chosen[u / (BLOCK / 16)] * BLOCK + (u % (BLOCK / 16)) * 16;
-      const int mine_l = label + (lane & 15), k8 = 8 * (lane >> 4);
-      const half_t* wp = a.W + (int64_t)(mine_l < a.N ? mine_l : a.N - 1) * a.ldw;
-      const half_t* xp = a.X + (int64_t)row * a.ldx;
-      float4v z = {0.f, 0.f, 0.f, 0.f};
-      for (int k0 = 0; k0 < a.K; k0 += 32 * STEPS) {
-        half8 wv[STEPS], xv[STEPS];
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-          const int k = k0 + 32 * j + k8;
-          wv[j] = *reinterpret_cast<const half8*>(wp + (k < a.K ? k : 0));
-          xv[j] = *reinterpret_cast<const half8*>(xp + (k < a.K ? k : 0));
-        }
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-          if (k0 + 32 * j >= a.K) break;
-          if (k0 + 32 * j + 32 > a.K) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              wv[j][e] = k0 + 32 * j + k8 < a.K ? wv[j][e] : (half_t)0.f;
-              xv[j][e] = k0 + 32 * j + k8 < a.K ? xv[j][e] : (half_t)0.f;
-            }
-          }
-          z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv[j], xv[j], z, 0, 0, 0);
-        }
-      }
-      if ((lane & 15) == 0) *reinterpret_cast<float4v*>(&score[u * 16 + 4 * (lane >> 4)]) = z;
+      const int part = u % (BLOCK / 16);
+      const float4v z = scores.score(a, row, (int)~(uint32_t)chosen[u / (BLOCK / 16)] * BLOCK, part, lane);
+      if ((lane & 15) == 0) *reinterpret_cast<float4v*>(&score[u / (BLOCK / 16) * BLOCK + Scores::place(part, lane)]) = z;
     }
     __syncthreads();
     // the K best of the blocks' labels and of what was there before

@@ -16,6 +16,7 @@
 #include "../../include/xfc_mi355x.h"
 #include "back_step.hpp"
 #include "back_wide.hpp"
+#include "launch.hpp"
 #include "pipe_core.hpp"
 #include "small_step.hpp"
 #include "tile_plan.hpp"
@@ -66,33 +67,6 @@ struct FwdLds {
 };
 static_assert(FwdCore::BN == fwd_tile_labels(FWD_128) && FwdCore::BM == fwd_tile_rows(FWD_128) && FwdCore64::BN == fwd_tile_labels(FWD_64) &&
               FwdCore64::BM == fwd_tile_rows(FWD_64), "tile_plan.hpp");
-
-constexpr int LOGIT_BLOCK = 32;
-// max of two packed halves each, and of three; an operand that is no number wins, so that a block with one can be told.
-// (Two wait states in front of the lane exchanges below, as for fold32.)
-__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t pk_max(const half8& v) {
-  const uint4v q = __builtin_bit_cast(uint4v, v);
-  return pk_max(pk_max(q[0], q[1], q[2]), q[3], q[3]);
-}
-__device__ __forceinline__ uint32_t pk_fold32(uint32_t a, uint32_t b) {
-  asm("s_nop 1" : "+v"(a), "+v"(b));
-  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-  return pk_max(r[0], r[1], r[1]);
-}
-__device__ __forceinline__ uint32_t pk_fold16(uint32_t a, uint32_t b) {
-  asm("s_nop 1" : "+v"(a), "+v"(b));
-  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-  return pk_max(r[0], r[1], r[1]);
-}
-__device__ __forceinline__ half_t pk_larger(uint32_t a) {  // of the two halves
-  const uint16_t h = (uint16_t)pk_max(a, a >> 16, a >> 16);
-  return __builtin_bit_cast(half_t, h);
-}
 
 struct FwdArgs {
   const half_t* X; int64_t ldx;     // M x K, K-contiguous
@@ -506,7 +480,7 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const double* __restr
 // ---------------------------------------------------------------------------------------------
 // top-K for 8 < K <= 8192: exact selection over rows of fp16 logits (one workgroup per row)
 // ---------------------------------------------------------------------------------------------
-constexpr int SEL_MAX_K = 8192;  // at most half the capacity of the larger sort buffer
+static_assert(SEL_MAX_K == 8192, "at most half the capacity of the larger sort buffer");
 constexpr int SEL_THREADS = 1024;
 constexpr int SEL_BINS = 2048;  // histogram over the top 11 bits of the 16-bit key
 // candidates that are sorted in LDS: 2048 for K <= 1024 (the reference's K = 100 lives here), 16384 (128 KB of
@@ -1313,62 +1287,6 @@ using namespace xfc;
 
 namespace {
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-int check_launch() {
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) {
-    fprintf(stderr, "xfc: kernel launch failed: %s\n", hipGetErrorString(e));
-    return XFC_ERR_HIP;
-  }
-  return XFC_OK;
-}
-
-constexpr int MAX_DEVICES = 64;
-int current_device() {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) dev = 0;
-  return dev;
-}
-
-constexpr int FULL_LDS = 160 * 1024;
-
-// Dynamic LDS above the default limit needs the attribute once per kernel and device.
-template <auto Kernel>
-hipError_t raise_lds_limit(int lds) {
-  static std::atomic<bool> raised[MAX_DEVICES];
-  const int dev = current_device();
-  if (lds <= 48 * 1024 || raised[dev].load(std::memory_order_acquire)) return hipSuccess;
-  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e == hipSuccess) raised[dev].store(true, std::memory_order_release);
-  return e;
-}
-
-// Launches Kernel and returns XFC_OK or XFC_ERR_HIP; nothing is launched when the LDS limit cannot be raised.
-template <auto Kernel, class A>
-int launch_k(dim3 g, dim3 b, int lds, hipStream_t st, const A& args) {
-  const hipError_t e = raise_lds_limit<Kernel>(lds);
-  if (e != hipSuccess) {
-    fprintf(stderr, "xfc: cannot raise the dynamic LDS limit to %d bytes: %s\n", lds, hipGetErrorString(e));
-    return XFC_ERR_HIP;
-  }
-  hipLaunchKernelGGL(Kernel, g, b, lds, st, args);
-  return check_launch();
-}
-
-int num_cus() {
-  static std::atomic<int> n[MAX_DEVICES];
-  const int dev = current_device();
-  int v = n[dev].load(std::memory_order_relaxed);
-  if (v == 0) {
-    int cnt = 0;
-    if (hipDeviceGetAttribute(&cnt, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cnt <= 0) cnt = 256;
-    v = cnt;
-    n[dev].store(v, std::memory_order_relaxed);
-  }
-  return v;
-}
-
 // Device address of g_static_scratch on the current device (each GPU holds its own copy at its own
 // address), looked up once per device; nullptr with the error printed if the lookup fails.
 void* static_scratch_ptr() {
@@ -1792,9 +1710,23 @@ int launch_select(int rows, const SelArgs& a, hipStream_t st) {
   return check_launch();
 }
 
-bool dims_ok(int64_t v) { return v >= 0 && v <= 0x7fffffff; }
-
 }  // namespace
+
+bool xfc::select_takes_maxima(int64_t K, int64_t n_blocks) {
+  return K <= SEL_BLOCKS_MAX_K && n_blocks >= 2 * K && n_blocks >= SEL_BLOCKS_MIN;
+}
+int xfc::select_rows(const half_t* logits, int64_t ldl, int rows, int L, int64_t numy, int K, const half_t* bmax, int64_t ldb,
+                     float* values, int64_t* indices, hipStream_t st) {
+  // sample every stride-th 16 KB block first when that still holds 16 K elements and points at about a
+  // thousand candidates at most (half the sort buffer)
+  const int cap = K <= SEL_SMALL_MAX_K ? SEL_CAP_SMALL : SEL_CAP_LARGE;
+  int stride = 1;
+  while (stride < 16 && (int64_t)K * stride * 2 <= cap / 2 && L / (stride * 2) >= 16 * (int64_t)K &&
+         L / (stride * 2) >= (int64_t)SEL_THREADS * 8 * 4)
+    stride *= 2;
+  const SelArgs sa = {logits, ldl, L, numy, K, stride, bmax, ldb, bmax ? ceil_div(L, LOGIT_BLOCK) : 0, values, indices};
+  return K <= SEL_SMALL_MAX_K ? launch_select<SEL_CAP_SMALL>(rows, sa, st) : launch_select<SEL_CAP_LARGE>(rows, sa, st);
+}
 
 extern "C" {
 
@@ -1894,7 +1826,7 @@ int xfc_init(void) {
   dw_all_limits(std::type_identity<DwCore>{});
   dw_all_limits(std::type_identity<DwCore128>{});
   (void)num_cus();
-  if (static_scratch_ptr() == nullptr) return XFC_ERR_HIP;
+  if (static_scratch_ptr() == nullptr || init_labels() != XFC_OK) return XFC_ERR_HIP;
   if (e != hipSuccess) {
     fprintf(stderr, "xfc: xfc_init failed: %s\n", hipGetErrorString(e));
     return XFC_ERR_HIP;
@@ -2470,7 +2402,7 @@ static int topk_impl(const void* X, int64_t ldx, const void* W, int64_t ldw, int
     const int64_t n_blocks = ceil_div(L, LOGIT_BLOCK), ldb = round_up(L, FwdWide::BM) / LOGIT_BLOCK;
     const size_t logits = (size_t)round_up((int64_t)((size_t)block * (size_t)ldl * 2), 16), maxima = (size_t)block * (size_t)ldb * 2;
     half_t* bmax = nullptr;
-    if (K <= SEL_BLOCKS_MAX_K && n_blocks >= 2 * (int64_t)K && n_blocks >= SEL_BLOCKS_MIN) {
+    if (select_takes_maxima(K, n_blocks)) {
       if (scratch && scratch_bytes >= maxima && aligned16(scratch)) bmax = (half_t*)scratch;
       else if (workspace_bytes >= logits + maxima) bmax = (half_t*)((unsigned char*)workspace + logits);
     }
@@ -2479,16 +2411,7 @@ static int topk_impl(const void* X, int64_t ldx, const void* W, int64_t ldw, int
       int rc = launch_fwd(fwd_plan(rows, L, d, false, num_cus()), FWD_LINEAR, (const half_t*)X + r0 * ldx, ldx, (const half_t*)W, ldw,
                           (half_t*)workspace, ldl, (int)rows, (int)L, (int)d, (int)L, 1.0f, 0.0f, st, NO_LOSS, bmax, ldb);
       if (rc) return rc;
-      // sample every stride-th 16 KB block first when that still holds 16 K elements and points at about a
-      // thousand candidates at most (half the sort buffer)
-      const int cap = K <= SEL_SMALL_MAX_K ? SEL_CAP_SMALL : SEL_CAP_LARGE;
-      int stride = 1;
-      while (stride < 16 && (int64_t)K * stride * 2 <= cap / 2 && L / (stride * 2) >= 16 * (int64_t)K &&
-             L / (stride * 2) >= (int64_t)SEL_THREADS * 8 * 4)
-        stride *= 2;
-      const SelArgs sa = {(const half_t*)workspace, ldl, (int)L, numy, K, stride, bmax, ldb, bmax ? (int)n_blocks : 0,
-                          values + r0 * K, indices + r0 * K};
-      rc = K <= SEL_SMALL_MAX_K ? launch_select<SEL_CAP_SMALL>((int)rows, sa, st) : launch_select<SEL_CAP_LARGE>((int)rows, sa, st);
+      rc = select_rows((const half_t*)workspace, ldl, (int)rows, (int)L, numy, K, bmax, ldb, values + r0 * K, indices + r0 * K, st);
       if (rc) return rc;
     }
     return XFC_OK;
@@ -2529,8 +2452,8 @@ static int topk_impl(const void* X, int64_t ldx, const void* W, int64_t ldw, int
     k.best = p.range < L ? reinterpret_cast<unsigned long long*>(a.bmax + (size_t)B * p.ldb) : nullptr;
     k.begin = l0 == 0; k.end = l0 + n == L;
     k.numy = numy; k.out_v = values; k.out_i = indices;
-    if (p.small) hipLaunchKernelGGL(topk_pick_kernel<SCORE_SMALL_BLOCK>, dim3((unsigned)B), dim3(512), 0, st, k);
-    else hipLaunchKernelGGL(topk_pick_kernel<SCORE_WIDE_BLOCK>, dim3((unsigned)B), dim3(512), 0, st, k);
+    if (p.small) hipLaunchKernelGGL(topk_pick_kernel<SCORE_SMALL_BLOCK>, dim3((unsigned)B), dim3(512), 0, st, k, HalfScores{});
+    else hipLaunchKernelGGL(topk_pick_kernel<SCORE_WIDE_BLOCK>, dim3((unsigned)B), dim3(512), 0, st, k, HalfScores{});
     if ((rc = check_launch())) return rc;
   }
   return XFC_OK;

@@ -368,6 +368,25 @@ class XFCLayer:
             self._g_live = True
         return G[:, : self.numy]
 
+    def preference_grad(self, embed, rowptr, chosen, rejected, reference: torch.Tensor | None = None,
+                        pair_weight: torch.Tensor | None = None, beta: float = 0.1, label_smoothing: float = 0.0,
+                        out: torch.Tensor | None = None):
+        """Adds the gradient of the preference loss of the batch's label pairs (renee_amd/preference.py) to the G that fwd_grad has
+        left, so that dx, dw_update, dw_accumulate and backward_pass carry it.  Returns (loss, margins)."""
+        from .preference import preference
+
+        x = self._x16(embed)
+        _require(out is not None or self._g_live, "preference_grad adds to the G of fwd_grad, and there is none")
+        loss, margin, _ = preference(x, self, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing,
+                                     g=self._g_view(x.shape[0], out))
+        return loss, margin
+
+    def quantize_labels(self):
+        """The label matrix in MX4 (renee_amd/mx4.py), from the fp32 master weights where the layer keeps them."""
+        from .mx4 import MX4Labels
+
+        return MX4Labels.from_weight(self.xfc_weight_master if self.master_weights else self.xfc_weight)
+
     def dx(self, bsz: int, grad_input: torch.Tensor | None = None, scale: float = 1.0,
            out: torch.Tensor | None = None) -> torch.Tensor:
         """grad_input = scale * G . W with W before the update (dl_base.py:602-608)."""

@@ -1,0 +1,245 @@
+"""Label matrices in MX4 against the format's definition in 64 bits (oracle/label_oracle.py): codes and scales to the last bit, logits
+and top-K at sizes that do not fill a unit, a step, a block or a row tile, blocks of zeros, NaNs and infinities."""
+import math
+
+import pytest
+import torch
+
+from oracle import label_oracle as O
+from renee_amd import MX4Labels, XFCLayer, mx4_dequantize, mx4_quantize
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def _matrix(L, d, dtype, seed, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(L, d, generator=g) * 0.02 * torch.exp2(spread * torch.randn(L, 1, generator=g))
+    return w.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,d", [(1, 8), (63, 32), (64, 64), (65, 72), (130, 128), (129, 200), (200, 768), (70, 136)])
+def test_codes_and_scales_are_those_of_the_definition(dev, L, d, dtype):
+    w = _matrix(L, d, dtype, L + d)
+    w[0] = 0                                        # a block of zeros
+    w[L // 2, :4] = torch.tensor([0.25, -0.75, 1.25, 2.5]).to(dtype)  # ties, under a block's largest of 4
+    w[L // 2, 4] = 4.0
+    w[L - 1, d - 1] = -7.5                          # beyond 6 after scaling
+    codes, scales = mx4_quantize(w.to(dev))
+    ec, es = O.pack(w)
+    assert torch.equal(scales.cpu(), es)
+    assert torch.equal(codes.cpu(), ec)
+    for out in DTYPES:
+        back = mx4_dequantize(codes, scales, L, d, out)
+        assert back.dtype == out and torch.equal(back.cpu(), O.rounded(w, 4).to(out))
+
+
+def test_codes_of_numbers_that_are_not_finite_and_of_the_smallest(dev):
+    w = _matrix(8, 96, torch.float32, 3)
+    w[1, 40] = float("inf")
+    w[2, 0] = float("nan")
+    w[3, 95] = -float("inf")
+    w[4, :32] = 2.0 ** -130 * torch.arange(32)      # the scale stops at 2^-127
+    w[5, :32] = 2.0 ** -125
+    w[6, 32:64] = 3e38
+    codes, scales = mx4_quantize(w.to(dev))
+    ec, es = O.pack(w)
+    assert torch.equal(scales.cpu(), es)
+    back = mx4_dequantize(codes, scales, 8, 96, torch.float32).cpu()
+    expect = O.rounded(w, 4).float()
+    assert torch.equal(torch.isnan(back), torch.isnan(expect))
+    assert torch.equal(torch.nan_to_num(back, nan=1.0), torch.nan_to_num(expect, nan=1.0))
+
+
+def test_strided_and_misaligned_weights(dev):
+    w = _matrix(100, 264, torch.float16, 5).to(dev)
+    for view in (w[:, :200], w[:, 3:203], w.t()[:100, :96], w[::3, 64:128]):
+        codes, scales = mx4_quantize(view)
+        ec, es = mx4_quantize(view.contiguous())
+        assert torch.equal(codes, ec) and torch.equal(scales, es)
+
+
+def _problem(B, L, d, bits, dtype, seed):
+    g = torch.Generator().manual_seed(seed + 1)
+    x = torch.randn(B, d, generator=g)
+    x = (x / x.norm(dim=1, keepdim=True)).to(dtype)
+    w = _matrix(L, d, torch.float16, seed, 0.3)
+    z = O.rounded(x, bits) @ O.rounded(w, 4).t()
+    return x, w, z
+
+
+def _logit_tolerance(x, w, bits):
+    """fp16 rounds by half a step, 2^-11 of the value or 2^-25; the sums in fp32 by 2^-24 of the magnitudes summed, once a product; and
+    with 8 bits the matrix pipe may drop 2^-14 of the largest of four neighbouring products, less than their sum."""
+    mass = O.rounded(x, bits).abs() @ O.rounded(w, 4).abs().t()
+    return mass * ((2.0 ** -14 if bits == 8 else 0.0) + 2.0 ** -24 * math.log2(2 * x.shape[1])) + 2.0 ** -25
+
+
+SIZES = [(1, 1, 8), (1, 65, 64), (3, 63, 32), (16, 200, 200), (17, 130, 136), (32, 64, 128), (33, 129, 768), (64, 257, 72), (65, 1000, 384),
+         (128, 640, 256), (129, 700, 96), (200, 300, 1024), (300, 5000, 64)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B,L,d", SIZES)
+def test_logits(dev, B, L, d, bits):
+    x, w, z = _problem(B, L, d, bits, DTYPES[(B + L) % 3], B + L + d)
+    labels = MX4Labels.from_weight(w.to(dev))
+    got = labels.xfc_forward(x.to(dev), embed_bits=bits).cpu().double()
+    tol = _logit_tolerance(x, w, bits) + z.abs() * 2.0 ** -11
+    assert got.shape == z.shape and bool(((got - z).abs() <= tol).all()), float(((got - z).abs() / tol).max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [2048, 4104, 8192])
+def test_logits_of_wide_embeddings(dev, d, bits):
+    x, w, z = _problem(40, 150, d, bits, torch.float16, d)
+    got = MX4Labels.from_weight(w.to(dev)).xfc_forward(x.to(dev), embed_bits=bits).cpu().double()
+    tol = _logit_tolerance(x, w, bits) + z.abs() * 2.0 ** -11
+    assert bool(((got - z).abs() <= tol).all())
+
+
+def test_logits_leave_what_lies_beside_them(dev):
+    x, w, z = _problem(37, 203, 72, 4, torch.float16, 9)
+    out = torch.full((40, 224), 7.0, dtype=torch.float16, device=dev)
+    MX4Labels.from_weight(w.to(dev)).xfc_forward(x.to(dev), out=out[:37, :203], embed_bits=4)
+    assert bool((out[37:] == 7).all()) and bool((out[:, 203:] == 7).all())
+    assert torch.equal(out[:37, :203].cpu(), z.half())  # 4 x 4 bits: sums are exact
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_row_or_label_that_is_no_number_stays_by_itself(dev, bits):
+    x, w, z = _problem(20, 100, 200, bits, torch.float16, 11)
+    x[3, 150] = float("inf")
+    w[70, 10] = float("nan")
+    got = MX4Labels.from_weight(w.to(dev)).xfc_forward(x.to(dev), embed_bits=bits).cpu()
+    bad = torch.zeros(20, 100, dtype=torch.bool)
+    bad[3], bad[:, 70] = True, True
+    assert torch.equal(torch.isnan(got), bad)
+
+
+# ---- top-K: with 4 bits sums are exact, so that values and labels are those of a stable sort -----------------------------------
+
+@pytest.mark.parametrize("K", [1, 5, 8, 9, 100])
+@pytest.mark.parametrize("B,L,d", [(1, 100, 64), (2, 131, 200), (16, 4097, 768), (33, 1000, 72), (100, 3001, 384), (130, 700, 128), (300, 2222, 96)])
+def test_topk_with_4_bits(dev, B, L, d, K):
+    x, w, z = _problem(B, L, d, 4, DTYPES[(B + K) % 3], B + L + d + K)
+    assert torch.equal(z.float().double(), z)
+    v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=4)
+    ev, ei = O.topk(z.half().double() if K > 8 else z, K)
+    assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
+
+
+@pytest.mark.parametrize("B,L,d,K", [(2, 70001, 64, 5), (40, 66000, 128, 100), (5, 140003, 64, 8), (3, 70001, 64, 3000)])
+def test_topk_of_many_labels(dev, B, L, d, K):
+    x, w, z = _problem(B, L, d, 4, torch.float16, L + K)
+    v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=4)
+    ev, ei = O.topk(z.half().double() if K > 8 else z, K)
+    assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
+
+
+@pytest.mark.parametrize("B,L,d,K", [(1, 1000, 768, 5), (40, 3001, 200, 8), (140, 2000, 64, 3), (20, 4000, 384, 50)])
+def test_topk_with_8_bits(dev, B, L, d, K):
+    """The labels' scores are within the product's tolerance of the definition's, none that was left out is above them by more than
+    twice that, and they are in order."""
+    x, w, z = _problem(B, L, d, 8, torch.float32, B + L + d + K)
+    v, i = (t.cpu() for t in MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K))
+    tol = _logit_tolerance(x, w, 8) + (z.abs() * 2.0 ** -11 if K > 8 else 0.0)
+    assert bool(((v.double() - z.gather(1, i)).abs() <= tol.gather(1, i)).all())
+    assert all(len(set(row.tolist())) == K for row in i)
+    order = v[:, :-1] - v[:, 1:]
+    assert bool((order >= 0).all()) and bool(((order > 0) | (i[:, :-1] < i[:, 1:])).all())
+    left = z.clone().scatter_(1, i, -math.inf)
+    assert bool((left <= v[:, -1:].double() + tol).all())
+
+
+def test_topk_ties_go_to_the_lower_label_and_constant_rows(dev):
+    w = torch.ones(300, 64, dtype=torch.float16)
+    w[7::50] = 2.0
+    x = torch.ones(3, 64, dtype=torch.float16)
+    x[1] = 0
+    for bits in (4, 8):
+        for K in (8, 20):
+            v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=bits)
+            ev, ei = O.topk((x.double() @ w.double().t()), K)
+            assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
+
+
+def test_topk_without_scores_and_clamped_labels(dev):
+    x, w, _ = _problem(4, 200, 64, 4, torch.float16, 21)
+    w[3:] = float("nan")
+    x[2] = float("nan")
+    z = O.rounded(x, 4) @ O.rounded(w, 4).t()
+    v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), 5, numy=150, embed_bits=4)
+    ev, ei = O.topk(z, 5)
+    assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), torch.where(ei < 0, 149, ei))
+
+
+def test_topk_rows_in_turns(dev):
+    """A workspace of 256 rows' logits takes 600 rows in three turns."""
+    from renee_amd._lib import check, lib
+
+    x, w, z = _problem(600, 3000, 64, 4, torch.float16, 33)
+    labels, xd = MX4Labels.from_weight(w.to(dev)), x.to(dev)
+    ev, ei = labels.topk(xd, 20, embed_bits=4)
+    need = lib().xfc_mx4_topk_workspace_bytes(256, 3000, 20)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    v, i = torch.empty_like(ev), torch.empty_like(ei)
+    check(lib().xfc_mx4_topk(xd.data_ptr(), 0, 64, labels.codes.data_ptr(), labels.scales.data_ptr(), 600, 3000, 64, 3000, 20, 4, v.data_ptr(),
+                             i.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream), "xfc_mx4_topk")
+    assert torch.equal(v, ev) and torch.equal(i, ei)
+    assert torch.equal(ei.cpu(), O.topk(z.half().double(), 20)[1])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("K", [5, 30])
+def test_replays_of_two_graphs_on_two_streams(dev, bits, K):
+    """Scratch belongs to a call: two captured calls of the same labels run beside each other, with new inputs between replays."""
+    x, w, _ = _problem(50, 3000, 128, bits, torch.float16, 41)
+    labels = MX4Labels.from_weight(w.to(dev))
+    xs = [x.to(dev), x.flip(0).contiguous().to(dev)]
+    eager = [labels.topk(t, K, embed_bits=bits) + (labels.xfc_forward(t, embed_bits=bits),) for t in xs]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for t in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(labels.topk(t, K, embed_bits=bits) + (labels.xfc_forward(t, embed_bits=bits),))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for outs in got:
+            for o in outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for outs, want in zip(got, eager):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_labels_of_a_layer(dev):
+    """quantize_labels follows the layer: the fp16 weights, or the fp32 ones where the layer keeps them; and a checkpoint of them."""
+    w = _matrix(500, 128, torch.float32, 51)
+    x = torch.randn(20, 128, generator=torch.Generator().manual_seed(1)).half()
+    for master in (False, True):
+        layer = XFCLayer(500, 128, 32, dev, weight=w.to(dev), master_weights=master)
+        labels = layer.quantize_labels()
+        assert torch.equal(labels.dequantize(torch.float32).cpu(), O.rounded(w if master else w.half(), 4).float())
+        # close to the layer's own logits: rounding weights to 4 bits is some 11 % of their norm
+        exact, rough = layer.xfc_forward(x.to(dev)).float(), labels.xfc_forward(x.to(dev)).float()
+        assert float((rough - exact).norm() / exact.norm()) < 0.25
+        again = MX4Labels.from_state_dict(labels.state_dict(), dev)
+        assert torch.equal(again.xfc_forward(x.to(dev)), labels.xfc_forward(x.to(dev)))
+
+
+def test_empty_calls(dev):
+    labels = MX4Labels.from_weight(torch.ones(70, 64, device=dev))
+    assert labels.xfc_forward(torch.empty(0, 64, device=dev)).shape == (0, 70)
+    assert labels.topk(torch.empty(0, 64, device=dev), 3)[1].shape == (0, 3)
+    none = MX4Labels.from_weight(torch.empty(0, 64, device=dev))
+    assert none.xfc_forward(torch.ones(3, 64, device=dev)).shape == (3, 0)
+    assert none.dequantize().shape == (0, 64)

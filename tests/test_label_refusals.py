@@ -1,0 +1,96 @@
+"""What MX4 label matrices and the preference loss refuse, on the CPU: nothing here reaches a device."""
+import ctypes
+
+import pytest
+import torch
+
+from renee_amd import MX4Labels, mx4_dequantize, mx4_quantize, preference
+from renee_amd._lib import lib
+
+ONE = ctypes.c_void_p(16)  # never dereferenced: every call below fails validation first
+F16, BF16, F32 = 0, 1, 2
+
+
+def _quantize(W=ONE, type=F16, ldw=64, L=10, d=64, codes=ONE, scales=ONE):
+    return lib().xfc_mx4_quantize(W, type, ldw, L, d, codes, scales, None)
+
+
+@pytest.mark.parametrize("how,code", [
+    (dict(W=None), 1), (dict(codes=None), 1), (dict(scales=None), 1), (dict(type=3), 1), (dict(L=-1), 1), (dict(d=0), 1), (dict(L=1 << 31), 1),
+    (dict(d=60), 3), (dict(ldw=68), 3), (dict(type=F32, ldw=66), 3), (dict(W=ctypes.c_void_p(24)), 3), (dict(codes=ctypes.c_void_p(8)), 3),
+    (dict(ldw=56), 6), (dict(L=0, W=None, codes=None, scales=None), 0)])
+def test_quantize(how, code):
+    assert _quantize(**how) == code
+    if "codes" not in how or how["codes"] is not None:
+        a = dict(W=ONE, type=F16, ldw=64, L=10, d=64, codes=ONE, scales=ONE) | how
+        assert lib().xfc_mx4_dequantize(a["codes"], a["scales"], a["L"], a["d"], a["W"], a["type"], a["ldw"], None) == code
+
+
+def _logits(X=ONE, type=F16, ldx=64, codes=ONE, scales=ONE, out=ONE, ldo=64, B=2, L=10, d=64, bits=8):
+    return lib().xfc_mx4_logits(X, type, ldx, codes, scales, out, ldo, B, L, d, bits, None)
+
+
+@pytest.mark.parametrize("how,code", [
+    (dict(X=None), 1), (dict(out=None), 1), (dict(bits=6), 1), (dict(B=-1), 1), (dict(d=0), 1), (dict(type=-1), 1), (dict(ldx=60), 3), (dict(ldo=12), 3),
+    (dict(out=ctypes.c_void_p(8)), 3), (dict(ldo=8), 6), (dict(ldx=56), 6), (dict(d=9096, ldx=9096), 7), (dict(d=16392, ldx=16392, bits=4), 7),
+    (dict(L=(1 << 30) + 1, ldo=1 << 31), 7), (dict(B=0, X=None), 0), (dict(L=0, codes=None), 0)])
+def test_logits(how, code):
+    assert _logits(**how) == code
+
+
+def _topk(X=ONE, ldx=64, B=2, L=1000, d=64, numy=1000, K=5, bits=4, values=ONE, indices=ONE, ws=ONE, nbytes=1 << 30):
+    return lib().xfc_mx4_topk(X, F16, ldx, ONE, ONE, B, L, d, numy, K, bits, values, indices, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("how,code", [
+    (dict(K=0), 1), (dict(K=8193, L=10000), 1), (dict(K=8, L=7), 1), (dict(numy=0), 1), (dict(values=None), 1), (dict(indices=None), 1), (dict(bits=5), 1),
+    (dict(ws=None), 4), (dict(nbytes=64), 4), (dict(K=9, nbytes=2 * 1000 * 2 - 16), 4), (dict(ws=ctypes.c_void_p(24)), 3), (dict(B=0), 0)])
+def test_topk(how, code):
+    assert _topk(**how) == code
+
+
+def test_workspaces():
+    h = lib()
+    assert h.xfc_mx4_code_bytes(65, 96) == 2 * 64 * 48 and h.xfc_mx4_scale_bytes(65, 96) == 2 * 64 * 4
+    assert h.xfc_mx4_code_bytes(-1, 64) == 0 and h.xfc_mx4_topk_workspace_bytes(4, 0, 1) == 0 and h.xfc_mx4_topk_workspace_bytes(4, 100, 9000) == 0
+    assert h.xfc_mx4_topk_workspace_bytes(300, 2812281, 8) < 300 * 2812281 * 4 // 31
+    for K in (8, 9):  # never shrinks with the rows
+        sizes = [h.xfc_mx4_topk_workspace_bytes(b, 70001, K) for b in range(1, 400)]
+        assert sizes == sorted(sizes)
+
+
+def _preference(X=ONE, type=F16, ldx=64, W=ONE, ldw=64, scales=None, L=10, d=64, rowptr=ONE, chosen=ONE, rejected=ONE, B=2, P=5, beta=0.1,
+                smoothing=0.0, loss=ONE, dX=ONE, dx_type=F32, lddx=64, G=None, ldg=0, ws=ONE, nbytes=1 << 20):
+    return lib().xfc_preference(X, type, ldx, W, ldw, scales, L, d, rowptr, chosen, rejected, None, None, B, P, beta, smoothing, 1.0, loss, None, dX,
+                                dx_type, lddx, G, ldg, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("how,code", [
+    (dict(X=None), 1), (dict(W=None), 1), (dict(rowptr=None), 1), (dict(chosen=None), 1), (dict(rejected=None), 1), (dict(loss=None), 1), (dict(L=0), 1),
+    (dict(d=0), 1), (dict(P=-1), 1), (dict(B=1 << 23), 1), (dict(dx_type=7), 1), (dict(smoothing=1.5), 1), (dict(smoothing=float("nan")), 1), (dict(beta=float("nan")), 1),
+    (dict(ldx=60), 3), (dict(ldw=60), 3), (dict(scales=ctypes.c_void_p(8)), 3), (dict(ldx=56), 6), (dict(ldw=56), 6), (dict(lddx=56), 6), (dict(G=ONE, ldg=9), 6),
+    (dict(d=4104, ldx=4104, ldw=4104, lddx=4104), 7), (dict(ws=None), 4), (dict(nbytes=16), 4), (dict(ws=ctypes.c_void_p(24)), 3)])
+def test_preference(how, code):
+    assert _preference(**how) == code
+
+
+def test_python_refuses_what_is_no_gpu_tensor():
+    w = torch.zeros(10, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        mx4_quantize(w)
+    with pytest.raises(RuntimeError, match="labels, dims"):
+        mx4_quantize(w[0])
+    codes, scales = torch.zeros(1, 64 * 32, dtype=torch.uint8), torch.zeros(1, 256, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        MX4Labels(codes, scales, 10, 64)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        mx4_dequantize(codes, scales, 10, 60)
+    with pytest.raises(TypeError, match="uint8"):
+        mx4_dequantize(codes.float(), scales, 10, 64)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        preference(torch.zeros(1, 64), w, i, i, i)
+    with pytest.raises(TypeError, match="float16"):
+        preference(torch.zeros(1, 64), w.float(), i, i, i)
+    with pytest.raises(RuntimeError, match="XFCLayer"):
+        preference(torch.zeros(1, 64), None, i, i, i)
