@@ -133,7 +133,9 @@ int check_product(const void* X, int type, int64_t ldx, const void* codes, const
   return XFC_OK;
 }
 
-int64_t mx_max_blocks(int64_t L) { return round_up(2 * (int64_t)ceil_div(L, MX_UNIT), 8); }  // maxima of a row, whole runs
+// maxima of a row: of 32 logits, of the units' sums, whole runs of them
+int64_t mx_half_maxima(int64_t L) { return 2 * (int64_t)ceil_div(L, MX_UNIT); }
+int64_t mx_maxima(int64_t L) { return round_up(ceil_div(L, MX_UNIT), 4); }
 
 }  // namespace
 
@@ -198,12 +200,12 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
 // K > 8: the logits of this many rows, and the maxima of their blocks
 static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
   const size_t logits = (size_t)rows * (size_t)round_up(L, 8) * 2;
-  return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_max_blocks(L) * 2 : 0);
+  return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_half_maxima(L) * 2 : 0);
 }
 
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K) {
   if (!dims_ok(B) || !dims_ok(L) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
-  if (K <= TOPK_MAX) return (size_t)B * (size_t)mx_max_blocks(L) * 4;
+  if (K <= TOPK_MAX) return (size_t)B * (size_t)mx_maxima(L) * 4;
   return mx_logit_rows_bytes(B, L, K);
 }
 
@@ -217,8 +219,8 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   if (!aligned16(workspace)) return XFC_ERR_ALIGN;
   const bool x8 = embed_bits == 8;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int64_t ldb = mx_max_blocks(L);
   if (K > TOPK_MAX) {
+    const int64_t ldb = mx_half_maxima(L);
     int64_t block = B;
     if (workspace_bytes < xfc_mx4_topk_workspace_bytes(B, L, K)) block = (int64_t)(workspace_bytes / xfc_mx4_topk_workspace_bytes(256, L, K)) * 256;
     const int64_t ldl = round_up(L, 8);
@@ -235,14 +237,15 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
     return XFC_OK;
   }
   float* const bmax = (float*)workspace;
-  rc = mx_product(MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d, 1, st);
+  const int64_t ldb = mx_maxima(L);
+  rc = mx_product(MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d, L >= (1 << 20) ? 4 : 1, st);
   if (rc) return rc;
   PickArgs k = {};
-  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, 32); k.N = (int)L; k.K = (int)d; k.topk = K;
+  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, MX_UNIT); k.N = (int)L; k.K = (int)d; k.topk = K;
   k.begin = k.end = 1; k.numy = numy; k.out_v = values; k.out_i = indices;
   auto pick = [&](auto s) {
     using S = decltype(s);
-    hipLaunchKernelGGL((topk_pick_kernel<32, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 18 KB at most
+    hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 18 KB at most
     return check_launch();
   };
   if (x8) return pick(MxScores<true>{X, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales});

@@ -267,13 +267,20 @@ __device__ __forceinline__ Float8 load8_of(const void* X, int type, int64_t at) 
 // ---------------------------------------------------------------------------------------------
 // products
 // ---------------------------------------------------------------------------------------------
+// A uniform address as the scalar half of a fetch's address: the compiler adds it up per lane otherwise.
+__device__ __forceinline__ const XFC_GLB uint8_t* scalar(const uint8_t* p) {
+  const XFC_GLB uint8_t* g = (const XFC_GLB uint8_t*)p;
+  asm volatile("" : "+s"(g));
+  return g;
+}
+
 enum MxOut { MX_LOGITS, MX_LOGITS_MAX, MX_MAXIMA };
 
 struct MxProductArgs {
   const void* X; int type; int64_t ldx;  // M rows of K
   const uint8_t* codes; const uint8_t* scales;
   half_t* out; int64_t ldo;              // logits
-  half_t* hmax; float* bmax; int64_t ldb; // maxima of blocks of 32 labels: of the logits as stored, of the sums
+  half_t* hmax; float* bmax; int64_t ldb; // maxima: of the logits as stored of 32 labels, of the sums of a unit
   int M, N, K;
   int units, blocks, steps;
   int tiles_m, slots;                    // row tiles; workgroups of a row tile on an XCD
@@ -281,10 +288,6 @@ struct MxProductArgs {
 };
 
 constexpr int MX_WAVES = 8, MX_SLOTS = 3;
-
-// rows of a workgroup: NT tiles of 16
-template <int NT, bool X8>
-constexpr int64_t mx_lds(int64_t d) { return (int64_t)mx_steps(d) * (NT * MxRows<X8>::FRAG + (NT + 3) / 4 * 256); }
 
 // A workgroup keeps its rows' fragments in the LDS and its waves, which never meet again, stream units of 64 labels past them, straight
 // into the A side's registers: MX_SLOTS - 1 steps on their way, across units.
@@ -317,8 +320,8 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     const bool rest = f_step == whole;
     const uint32_t at = rest ? at_rest : at_whole, tile = rest ? (uint32_t)wide * 256 : 1024u;
 #pragma unroll
-    for (int t = 0; t < MX_TILES; ++t) to.w[t] = *reinterpret_cast<const int4v*>(c + t * tile + at);
-    to.s = *reinterpret_cast<const uint32_t*>(s + (uint32_t)lane * 4);
+    for (int t = 0; t < MX_TILES; ++t) to.w[t] = *reinterpret_cast<const XFC_GLB int4v*>(scalar(c + t * tile) + at);
+    to.s = *reinterpret_cast<const XFC_GLB uint32_t*>(scalar(s) + (uint32_t)lane * 4);
     if (++f_step == a.steps) {
       f_step = 0;
       if (next(f_unit) < a.units) f_unit = next(f_unit);
@@ -340,29 +343,51 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
   __syncthreads();
 
   float4v acc[MX_TILES][NT];
-  [[maybe_unused]] float best[(NT + 1) / 2][4];
+  [[maybe_unused]] float4v best[NS];  // of up to four units in a row
   int step = 0;
 
-  auto multiply = [&](const Slot& w, auto first) {
-    uint32_t sb[NS];
+  // Row fragments run AHEAD of the MFMAs that read them, over the steps' ends: a step's first ones are read under the last MFMAs of the one before.
+  constexpr int RING = NT < 4 ? NT : 4, AHEAD = (RING + 1) / 2;
+  int8v ring[RING];
+  uint32_t sb[2][NS];
+  auto read_rows = [&](int of, auto jt) { ring[decltype(jt)::value % RING] = Rows::get(frags + (of * NT + decltype(jt)::value) * Rows::FRAG, lane); };
+  auto read_scales = [&](int of, uint32_t (&to)[NS]) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) sb[n] = *reinterpret_cast<const uint32_t*>(row_scales + ((step * NS + n) * 64 + lane) * 4);
+    for (int n = 0; n < NS; ++n) to[n] = *reinterpret_cast<const uint32_t*>(row_scales + ((of * NS + n) * 64 + lane) * 4);
+  };
+  [&]<int... J>(std::integer_sequence<int, J...>) { (read_rows(0, std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, AHEAD>{});
+  read_scales(0, sb[0]);
+  auto multiply = [&](const Slot& w, auto first) {
+    const int after = step + 1 == a.steps ? 0 : step + 1;
+    read_scales(after, sb[1]);
     auto row_tile = [&](auto jt) {
-      constexpr int J = decltype(jt)::value;
-      const int8v b = Rows::get(frags + (step * NT + J) * Rows::FRAG, lane);
+      constexpr int J = decltype(jt)::value, NEXT = (J + AHEAD) % NT;
+      const int8v b = ring[J % RING];
+      read_rows(J + AHEAD < NT ? step : after, std::integral_constant<int, NEXT>{});
       auto tile = [&](auto tt) {
         constexpr int T = decltype(tt)::value;
-        acc[T][J] = mx_mfma<X8, T, J % 4>(w.w[T], w.s, b, sb[J / 4], decltype(first)::value ? float4v{0.f, 0.f, 0.f, 0.f} : acc[T][J]);
+        acc[T][J] = mx_mfma<X8, T, J % 4>(w.w[T], w.s, b, sb[0][J / 4], decltype(first)::value ? float4v{0.f, 0.f, 0.f, 0.f} : acc[T][J]);
       };
       [&]<int... T>(std::integer_sequence<int, T...>) { (tile(std::integral_constant<int, T>{}), ...); }(std::make_integer_sequence<int, MX_TILES>{});
+      if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
     };
     [&]<int... J>(std::integer_sequence<int, J...>) { (row_tile(std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, NT>{});
+#pragma unroll
+    for (int n = 0; n < NS; ++n) sb[0][n] = sb[1][n];
   };
 
   auto epilogue = [&]() {
+    // (Made anew each time: kept over the loop, the rows' addresses would take the registers of the fragments under way.)
+    int lane_now = lane;
+    asm volatile("" : "+v"(lane_now));
+    const int i = lane_now & 15, q = lane_now >> 4;
     const int label0 = unit * MX_UNIT;
     const bool edge = label0 + MX_UNIT > a.N;
     if constexpr (OUT == MX_MAXIMA) {
+      // The maxima below are inline asm, in front of which the compiler puts no wait states: the last MFMAs' results are waited for here.
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 15\n\ts_nop 15");
+      __builtin_amdgcn_sched_barrier(0);
       if (edge) {
 #pragma unroll
         for (int t = 0; t < MX_TILES; ++t)
@@ -373,31 +398,30 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
             for (int j = 0; j < NT; ++j) acc[t][j][r] = in ? acc[t][j][r] : __builtin_nanf("");
           }
       }
-      auto largest = [&](int p, int j) {  // of this lane's eight labels
-        const float4v lo = acc[2 * p][j], hi = acc[2 * p + 1][j];
-        return fmaxf(fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])), fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])));
+      auto largest = [&](int j) {  // of this lane's sixteen labels
+        j = j < NT ? j : NT - 1;
+        float m = acc[0][j][0];
+#pragma unroll
+        for (int e = 1; e < 15; e += 2) m = max3_num(m, acc[e >> 2][j][e & 3], acc[(e + 1) >> 2][j][(e + 1) & 3]);
+        return max_num(m, acc[3][j][3]);
       };
       const int r4 = unit & (run - 1);
 #pragma unroll
-      for (int j2 = 0; j2 < (NT + 1) / 2; ++j2) {
-        // lane group g ends up with block g / 2 of row tile 2 j2 + g % 2
-        const int j1 = 2 * j2 + 1 < NT ? 2 * j2 + 1 : 2 * j2;
-        const float m = fold16(fold32(largest(0, 2 * j2), largest(1, 2 * j2)), fold32(largest(0, j1), largest(1, j1)));
+      for (int n = 0; n < NS; ++n) {
+        // lane group g ends up with row tile 4 n + g
+        const float m = fold16(fold32(largest(4 * n), largest(4 * n + 2)), fold32(largest(4 * n + 1), largest(4 * n + 3)));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) best[j2][r] = r4 == r ? m : best[j2][r];
+        for (int r = 0; r < 4; ++r) best[n][r] = r4 == r ? m : best[n][r];
       }
       const int after = next(unit);
       if (after != unit + 1 || run == 1 || after >= a.units) {
-        const int64_t first = 2 * (int64_t)(unit - r4);
 #pragma unroll
-        for (int j2 = 0; j2 < (NT + 1) / 2; ++j2) {
-          const int row = row0 + 32 * j2 + 16 * (q & 1) + i;
-          if (2 * j2 + (q & 1) >= NT || row >= a.M) continue;
-          float* const to = a.bmax + (int64_t)row * a.ldb + first;
-          if (run == 1) to[q >> 1] = best[j2][0];
-          else
-#pragma unroll
-            for (int r = 0; r < 4; ++r) to[2 * r + (q >> 1)] = best[j2][r];
+        for (int n = 0; n < NS; ++n) {
+          const int row = row0 + 64 * n + lane_now;
+          if (4 * n + q >= NT || row >= a.M) continue;
+          float* const to = a.bmax + (int64_t)row * a.ldb + (unit - r4);
+          if (run == 1) *to = best[n][0];
+          else *reinterpret_cast<float4v*>(to) = best[n];
         }
       }
     } else {
@@ -448,14 +472,13 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
           step = 0;
           unit = next(unit);
         }
-        fetch(slot[s]);
       }
+      fetch(slot[s]);  // (whatever way was taken: else the compiler could not tell how many are on their way, and would wait for all)
     }
   }
 }
 
-// How topk_pick_kernel forms the scores of sixteen labels again: blocks of 32 labels are half units, the sixteen are one of their two
-// tiles.  The row, quantised once, stands in all sixteen columns; the MFMAs and their order are those of mx4_product_kernel.
+// How topk_pick_kernel forms the scores of sixteen labels again: blocks are units, the sixteen are one of their four tiles.  The row, quantised once, stands in all sixteen columns; the MFMAs and their order are those of mx4_product_kernel.
 template <bool X8>
 struct MxScores {
   const void* X; int type; int64_t ldx;
@@ -483,19 +506,18 @@ struct MxScores {
       if (part == 0) s[STEP_BYTES - 16 + block] = (unsigned char)byte;
     }
   }
-  static __device__ __forceinline__ int place(int part, int lane) { return 8 * (lane >> 4) + 4 * part; }
+  static __device__ __forceinline__ int place(int part, int lane) { return mx_label(part, 4 * (lane >> 4)); }
   __device__ __forceinline__ float4v score(const PickArgs& a, int, int first, int part, int lane) const {
     const int blocks = mx_blocks(a.K), steps = mx_steps(a.K), i = lane & 15, q = lane >> 4;
     const int64_t unit = first / MX_UNIT;
-    const int p = (first % MX_UNIT) / 32;
     const uint8_t* const c = codes + unit * mx_code_bytes(a.K);
     const uint8_t* const s = scales + unit * mx_scale_bytes(a.K);
     const unsigned char* const at = room();
     float4v z = {0.f, 0.f, 0.f, 0.f};
     for (int step = 0; step < steps; ++step) {
       const int wide = blocks - 4 * step < 4 ? blocks - 4 * step : 4;
-      const int4v w = *reinterpret_cast<const int4v*>(c + mx_code_at(2 * p + part, i, 4 * step + (q < wide ? q : wide - 1), blocks));
-      const uint32_t sa = *reinterpret_cast<const uint32_t*>(s + step * 256 + lane * 4) >> (8 * (2 * p + part));
+      const int4v w = *reinterpret_cast<const int4v*>(c + mx_code_at(part, i, 4 * step + (q < wide ? q : wide - 1), blocks));
+      const uint32_t sa = *reinterpret_cast<const uint32_t*>(s + step * 256 + lane * 4) >> (8 * part);
       const unsigned char* const x = at + step * STEP_BYTES;
       int8v b;
       if constexpr (X8) {

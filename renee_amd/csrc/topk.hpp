@@ -405,7 +405,8 @@ template <int BLOCK, class Scores = HalfScores>
 __global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a, Scores scores) {
   constexpr int NW = 8, LISTS = NW * TOPK_MAX;
   constexpr int FETCH = 8;  // maxima on their way
-  static_assert(TOPK_MAX * BLOCK <= 512 - TOPK_MAX, "one candidate per thread");
+  static_assert(TOPK_MAX * BLOCK <= 512, "one candidate per thread");
+  constexpr bool APART = TOPK_MAX * BLOCK > 512 - TOPK_MAX;  // no thread is left for what was kept
   __shared__ unsigned long long list[LISTS], chosen[TOPK_MAX], kept[TOPK_MAX];
   __shared__ float score[TOPK_MAX * BLOCK];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -496,10 +497,14 @@ __global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a, Scores score
     if (tid < n_sel * BLOCK) {
       const int64_t label = (int64_t)(int)~(uint32_t)chosen[tid / BLOCK] * BLOCK + tid % BLOCK;
       if (label < a.N) key = topk_entry(score[tid], (uint32_t)(a.first + label));
-    } else if (tid >= 512 - TOPK_MAX) {
+    } else if (!APART && tid >= 512 - TOPK_MAX) {
       key = kept[tid - (512 - TOPK_MAX)];
     }
     bound = chosen[K - 1];
+    if constexpr (APART) {
+      top_of_all(key, chosen);
+      key = tid < K ? chosen[tid] : tid >= TOPK_MAX && tid < TOPK_MAX + K ? kept[tid - TOPK_MAX] : 0ull;
+    }
     top_of_all(key, kept);
     // (a block whose maximum is -inf may hold nothing but scores that are no numbers: then there may be more elsewhere)
     if (kept[K - 1] != 0 || bound == 0) break;

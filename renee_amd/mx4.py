@@ -14,22 +14,50 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .xfc import _require, _round_up, _stream
+from .xfc import _require, _round_up
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # xfc_type
 
 
+class _On:
+    """The device of a call: made current where it is not, with its current stream's handle.  (torch.cuda.device and current_stream take
+    some 6 us of host time, as much as the smallest of these kernels.)"""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *_):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
 def _rows(t: torch.Tensor, device: torch.device, dims: int, what: str) -> torch.Tensor:
     """A (rows, dims) matrix as the kernels read it: one of TYPES, on `device`, rows that begin on 16 bytes."""
-    _require(isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[1] == dims, f"{what} must be (rows, {dims})")
-    _require(t.dtype in TYPES, f"{what} must be float16, bfloat16 or float32", TypeError)
-    t = t.detach().to(device)
-    whole = t.stride(1) == 1 and t.stride(0) >= dims and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0
-    return t if whole else t.clone(memory_format=torch.contiguous_format)
+    if not (isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[1] == dims):
+        raise RuntimeError(f"{what} must be (rows, {dims})")
+    if t.dtype not in TYPES:
+        raise TypeError(f"{what} must be float16, bfloat16 or float32")
+    if t.device != device:
+        t = t.detach().to(device)
+    ld, one = t.stride()
+    if one == 1 and ld >= dims and ld * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _check_dims(dims: int) -> None:
     _require(dims > 0 and dims % 8 == 0, "dims must be a multiple of 8")
+
+
+def _unit_bytes(dims: int):
+    """Bytes of codes and of scales of 64 labels (xfc_mx4_code_bytes, xfc_mx4_scale_bytes)."""
+    return 1024 * ((dims + 31) // 32), 256 * ((dims + 127) // 128)
 
 
 def mx4_quantize(weight: torch.Tensor):
@@ -39,12 +67,12 @@ def mx4_quantize(weight: torch.Tensor):
     numy, dims = weight.shape
     _check_dims(dims)
     weight = _rows(weight, weight.device, dims, "weight")
-    L, units = lib(), (numy + 63) // 64
-    codes = torch.empty(units, L.xfc_mx4_code_bytes(64, dims), dtype=torch.uint8, device=weight.device)
-    scales = torch.empty(units, L.xfc_mx4_scale_bytes(64, dims), dtype=torch.uint8, device=weight.device)
-    with torch.cuda.device(weight.device):
-        rc = L.xfc_mx4_quantize(weight.data_ptr(), TYPES[weight.dtype], weight.stride(0), numy, dims, codes.data_ptr(),
-                                scales.data_ptr(), _stream(weight))
+    units, (code, scale) = (numy + 63) // 64, _unit_bytes(dims)
+    codes = torch.empty(units, code, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(units, scale, dtype=torch.uint8, device=weight.device)
+    with _On(weight.device) as stream:
+        rc = lib().xfc_mx4_quantize(weight.data_ptr(), TYPES[weight.dtype], weight.stride(0), numy, dims, codes.data_ptr(), scales.data_ptr(),
+                                    stream)
     check(rc, "xfc_mx4_quantize")
     return codes, scales
 
@@ -52,12 +80,14 @@ def mx4_quantize(weight: torch.Tensor):
 def _check_codes(codes: torch.Tensor, scales: torch.Tensor, numy: int, dims: int) -> None:
     _check_dims(dims)
     _require(numy >= 0, "numy must not be negative")
-    L, units = lib(), (numy + 63) // 64
-    for t, row, what in ((codes, L.xfc_mx4_code_bytes(64, dims), "codes"), (scales, L.xfc_mx4_scale_bytes(64, dims), "scales")):
-        _require(isinstance(t, torch.Tensor) and t.dtype == torch.uint8, f"{what} must be a uint8 tensor", TypeError)
-        _require(t.is_cuda, "expected a GPU tensor")
-        _require(tuple(t.shape) == (units, row) and t.is_contiguous() and t.data_ptr() % 16 == 0,
-                 f"{what} of {numy} labels x {dims} dims must be a contiguous ({units}, {row}) tensor that begins on 16 bytes")
+    units = (numy + 63) // 64
+    for t, row, what in zip((codes, scales), _unit_bytes(dims), ("codes", "scales")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8:
+            raise TypeError(f"{what} must be a uint8 tensor")
+        if not t.is_cuda:
+            raise RuntimeError("expected a GPU tensor")
+        if t.shape != (units, row) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise RuntimeError(f"{what} of {numy} labels x {dims} dims must be a contiguous ({units}, {row}) tensor that begins on 16 bytes")
     _require(codes.device == scales.device, "codes and scales must share a device")
 
 
@@ -66,8 +96,8 @@ def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, numy: int, dims: i
     _check_codes(codes, scales, numy, dims)
     _require(dtype in TYPES, "dtype must be float16, bfloat16 or float32", TypeError)
     out = torch.empty(numy, dims, dtype=dtype, device=codes.device)
-    with torch.cuda.device(codes.device):
-        rc = lib().xfc_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), numy, dims, out.data_ptr(), TYPES[dtype], dims, _stream(out))
+    with _On(codes.device) as stream:
+        rc = lib().xfc_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), numy, dims, out.data_ptr(), TYPES[dtype], dims, stream)
     check(rc, "xfc_mx4_dequantize")
     return out
 
@@ -93,19 +123,23 @@ class MX4Labels:
         """Logits embed . W^T in float16 (dl_base.py:568-573), into `out` if it is given."""
         x = _rows(embed, self.device, self.dims, "embed")
         _require(embed_bits in (4, 8), "embed_bits must be 4 or 8", ValueError)
-        bsz = x.shape[0]
+        bsz, ld = x.shape[0], _round_up(self.numy, 8)
         if out is None:
-            out = torch.empty(bsz, _round_up(self.numy, 8), dtype=torch.float16, device=self.device)[:, :self.numy]
-        _require(out.dtype == torch.float16 and tuple(out.shape) == (bsz, self.numy) and out.device == self.device,
-                 "out must be float16 (batch, numy) on the labels' device")
+            out = torch.empty(bsz, ld, dtype=torch.float16, device=self.device)
+            if ld != self.numy:
+                out = out[:, :self.numy]
+        else:
+            _require(out.dtype == torch.float16 and out.shape == (bsz, self.numy) and out.device == self.device,
+                     "out must be float16 (batch, numy) on the labels' device")
+            _require(out.numel() == 0 or (out.stride(1) == 1 or self.numy == 1) and (out.stride(0) % 8 == 0 and out.stride(0) >= self.numy or bsz == 1) and
+                     out.data_ptr() % 16 == 0, "out must have a row stride that is a multiple of 8 and begin on 16 bytes")
+            if bsz > 1:
+                ld = out.stride(0)
         if out.numel() == 0:
             return out
-        _require((out.stride(1) == 1 or self.numy == 1) and (out.stride(0) % 8 == 0 and out.stride(0) >= self.numy or bsz == 1) and
-                 out.data_ptr() % 16 == 0, "out must have a row stride that is a multiple of 8 and begin on 16 bytes")
-        ldo = out.stride(0) if bsz > 1 else _round_up(self.numy, 8)
-        with torch.cuda.device(self.device):
+        with _On(self.device) as stream:
             rc = lib().xfc_mx4_logits(x.data_ptr(), TYPES[x.dtype], x.stride(0), self.codes.data_ptr(), self.scales.data_ptr(),
-                                      out.data_ptr(), ldo, bsz, self.numy, self.dims, embed_bits, _stream(x))
+                                      out.data_ptr(), ld, bsz, self.numy, self.dims, embed_bits, stream)
         check(rc, "xfc_mx4_logits")
         return out
 
@@ -125,10 +159,10 @@ class MX4Labels:
         if need > 1 << 32 and K > 8:  # the logits of some rows at a time
             need = max(min(need, 1 << 32), L.xfc_mx4_topk_workspace_bytes(min(bsz, 256), self.numy, K))
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        with torch.cuda.device(self.device):
+        with _On(self.device) as stream:
             rc = L.xfc_mx4_topk(x.data_ptr(), TYPES[x.dtype], x.stride(0), self.codes.data_ptr(), self.scales.data_ptr(), bsz, self.numy,
                                 self.dims, self.numy if numy is None else int(numy), int(K), embed_bits, values.data_ptr(),
-                                indices.data_ptr(), ws.data_ptr(), need, _stream(x))
+                                indices.data_ptr(), ws.data_ptr(), need, stream)
         check(rc, "xfc_mx4_topk")
         return values, indices
 

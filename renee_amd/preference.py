@@ -21,17 +21,22 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .mx4 import MX4Labels, TYPES, _rows
-from .xfc import XFCLayer, _require, _stream
+from .mx4 import MX4Labels, TYPES, _On, _rows
+from .xfc import XFCLayer, _require
 
 
 def _list(t: torch.Tensor | None, dtype: torch.dtype, n: int, device: torch.device, what: str) -> torch.Tensor | None:
     if t is None:
         return None
-    _require(isinstance(t, torch.Tensor) and t.dim() == 1, f"{what} must be a 1-D tensor")
-    _require(t.dtype == dtype, f"{what} must be {dtype}", TypeError)
-    _require(n < 0 or t.numel() == n, f"{what} must have {n} entries")
-    return t.detach().to(device).contiguous()
+    if not (isinstance(t, torch.Tensor) and t.dim() == 1):
+        raise RuntimeError(f"{what} must be a 1-D tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}")
+    if n >= 0 and t.shape[0] != n:
+        raise RuntimeError(f"{what} must have {n} entries")
+    if t.device != device:
+        t = t.to(device)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _labels(labels):
@@ -52,10 +57,10 @@ def _labels(labels):
 def preference(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.Tensor, rejected: torch.Tensor,
                reference: torch.Tensor | None = None, pair_weight: torch.Tensor | None = None, beta: float = 0.1,
                label_smoothing: float = 0.0, scale: float = 1.0, g: torch.Tensor | None = None, grad_dtype: torch.dtype = torch.float32,
-               need_grad: bool = True):
+               need_grad: bool = True, need_margin: bool = True):
     """(loss, margin, grad_input) of the pairs, outside autograd: the summed loss (one float32), the pairs' margins (float32) and scale
     times the gradient of `embed`, or None with `g`, a G buffer of a training step to whose entries the pairs' gradient is added
-    instead.
+    instead.  need_grad and need_margin leave out what is not wanted.
 
     rowptr int32[batch + 1], chosen and rejected int32[pairs] (coo_to_csr makes such lists); reference and pair_weight float32[pairs].
     A pair with a label that is none (-1, say) or weight 0 is not there, whatever else it holds."""
@@ -75,10 +80,10 @@ def preference(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.
     if g is not None:
         _require(g.dtype == torch.float16 and g.dim() == 2 and g.device == device and g.shape[0] == bsz and g.shape[1] >= numy and
                  (g.stride(1) == 1 or g.shape[1] <= 1) and (g.stride(0) >= numy or bsz <= 1), "g must be float16 (batch, numy) on the labels' device")
-    loss = torch.empty(1, dtype=torch.float32, device=device)
-    margin = torch.empty(P, dtype=torch.float32, device=device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    margin = torch.empty(P, dtype=torch.float32, device=device) if need_margin else None
     grad = torch.empty(bsz, dims, dtype=grad_dtype, device=device) if g is None and need_grad else None
-    if bsz == 0:
+    if bsz == 0 and need_margin:
         margin.zero_()
     L = lib()
     need = L.xfc_preference_workspace_bytes(bsz, P, dims)
@@ -87,13 +92,13 @@ def preference(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.
     def at(t):
         return None if t is None else t.data_ptr()
 
-    with torch.cuda.device(device):
-        rc = L.xfc_preference(x.data_ptr(), TYPES[x.dtype], x.stride(0) if bsz > 1 else dims, W.data_ptr(), ldw, at(scales), numy, dims, at(rowptr),
-                              at(chosen), at(rejected), at(reference), at(pair_weight), bsz, P, float(beta), float(label_smoothing),
-                              float(scale), loss.data_ptr(), margin.data_ptr(), at(grad), TYPES[grad_dtype], dims, at(g),
-                              0 if g is None else g.stride(0) if bsz > 1 else max(g.stride(0), numy), ws.data_ptr(), need, _stream(x))
+    with _On(device) as stream:
+        rc = L.xfc_preference(x.data_ptr(), TYPES[x.dtype], x.stride(0) if bsz > 1 else dims, W.data_ptr(), ldw, at(scales), numy, dims,
+                              rowptr.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), at(reference), at(pair_weight), bsz, P, beta,
+                              label_smoothing, scale, loss.data_ptr(), at(margin), at(grad), TYPES[grad_dtype], dims, at(g),
+                              0 if g is None else g.stride(0) if bsz > 1 else max(g.stride(0), numy), ws.data_ptr(), need, stream)
     check(rc, "xfc_preference")
-    return loss.reshape(()), margin, grad
+    return loss, margin, grad
 
 
 def pair_margins(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.Tensor, rejected: torch.Tensor) -> torch.Tensor:
@@ -104,18 +109,15 @@ def pair_margins(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torc
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, embed, labels, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing, scale):
-        ctx.embed_device = embed.device
-        loss, _, grad = preference(embed, labels, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing, scale,
-                                   grad_dtype=embed.dtype, need_grad=ctx.needs_input_grad[0])
-        if grad is not None:
-            ctx.save_for_backward(grad)
+        loss, _, ctx.grad = preference(embed, labels, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing, scale,
+                                       grad_dtype=embed.dtype, need_grad=ctx.needs_input_grad[0], need_margin=False)
+        ctx.device = embed.device
         return loss
 
     @staticmethod
     def backward(ctx, grad_out):
-        (grad,) = ctx.saved_tensors
-        g = (grad * grad_out.to(device=grad.device, dtype=torch.float32)).to(device=ctx.embed_device, dtype=grad.dtype)
-        return (g,) + (None,) * 9
+        grad = ctx.grad * grad_out
+        return grad if grad.device == ctx.device else grad.to(ctx.device), None, None, None, None, None, None, None, None, None
 
 
 def preference_loss(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.Tensor, rejected: torch.Tensor,
