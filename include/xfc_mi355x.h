@@ -326,13 +326,14 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
  *   loss = sum weight[p] * (-(1 - smoothing) log sigmoid(beta margin) - smoothing log sigmoid(-beta margin))       (one float)
  *   slope[p] = d loss / d margin = weight[p] * beta * (sigmoid(beta margin) - (1 - smoothing))
  * and its gradient, in either form or both:
- *   dX[b] = scale * sum slope[p] (W[chosen] - W[rejected])           (rows of d, dx_type; rows without pairs are written as zero)
+ *   dX[b] = scale * sum slope[p] (W[chosen] - W[rejected])           (rows of d, dx_type, 16-byte aligned; without pairs zero)
  *   G[b][chosen] += slope[p], G[b][rejected] -= slope[p]             (fp16, as xfc_fwd_grad_* leaves it: xfc_dx and xfc_dw_* then
  *                                                                    carry the pairs too; entries of one row and label are added up in fp32
  *                                                                    and rounded once per 512 pairs of the row)
  * X: fp16, bf16 or fp32.  W: fp16 rows, or with scales non-NULL MX4 codes (ldw is not used).  reference, weight, margin, dX, G may be NULL
  * (0, 1, not wanted).  A pair with a label outside [0, L) or weight 0 is not there, whatever else it holds: its margin is 0, and so is
- * that of pairs which no row has.  Results do not depend on anything but the arguments: no atomics.  d <= 4096, a multiple of 8.
+ * that of pairs which no row has.  Row pointers that do not ascend give an unspecified result for the rows of these pairs.  Results do not depend on
+ * anything but the arguments: no atomics.  d <= 4096, a multiple of 8.
  */
 size_t xfc_preference_workspace_bytes(int64_t B, int64_t P, int64_t d);
 int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t ldw, const void* scales, int64_t L, int64_t d,

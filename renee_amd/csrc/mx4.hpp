@@ -75,6 +75,24 @@ __device__ __forceinline__ Float8 load8(const void* p) {
   }
   return f;
 }
+template <int TYPE>
+__device__ __forceinline__ void store8(void* p, const Float8& f) {
+  if constexpr (TYPE == XFC_F32) {
+    reinterpret_cast<float4v*>(p)[0] = float4v{f.v[0], f.v[1], f.v[2], f.v[3]};
+    reinterpret_cast<float4v*>(p)[1] = float4v{f.v[4], f.v[5], f.v[6], f.v[7]};
+  } else if constexpr (TYPE == XFC_BF16) {
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    bf16x8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (__bf16)f.v[e];
+    *reinterpret_cast<bf16x8*>(p) = h;
+  } else {
+    half8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (half_t)f.v[e];
+    *reinterpret_cast<half8*>(p) = h;
+  }
+}
 constexpr int type_bytes(int type) { return type == XFC_F32 ? 4 : 2; }
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {  // over four neighbouring lanes
@@ -198,22 +216,7 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(MxArgs a) {
     const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + ((t * 16 + row) * wide + block) * 16 + part * 4);
     const Float8 f = from_fp4(c, scale_value((bytes >> (8 * t)) & 255u));
     if (label >= a.L) continue;
-    char* const to = reinterpret_cast<char*>(a.out) + (label * a.ldw + k) * type_bytes(TYPE);
-    if constexpr (TYPE == XFC_F32) {
-      reinterpret_cast<float4v*>(to)[0] = float4v{f.v[0], f.v[1], f.v[2], f.v[3]};
-      reinterpret_cast<float4v*>(to)[1] = float4v{f.v[4], f.v[5], f.v[6], f.v[7]};
-    } else if constexpr (TYPE == XFC_BF16) {
-      typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-      bf16x8 h;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = (__bf16)f.v[e];
-      *reinterpret_cast<bf16x8*>(to) = h;
-    } else {
-      half8 h;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = (half_t)f.v[e];
-      *reinterpret_cast<half8*>(to) = h;
-    }
+    store8<TYPE>(reinterpret_cast<char*>(a.out) + (label * a.ldw + k) * type_bytes(TYPE), f);
   }
 }
 

@@ -5,9 +5,11 @@
 //   slope = a beta (sigmoid(beta m) - (1 - e))  = d loss / d m
 //   dX_b = scale sum slope (w_c - w_r);         or G[b][c] += slope, G[b][r] -= slope, from which dX and dW follow
 //
-// Bound by fetching two rows of labels per pair from anywhere.  A wave takes pairs of one row, four at a time, whole rows of
-// weights in its registers; the difference that makes the margin makes the gradient too, so rows are fetched once.  Everything is summed
-// in fp32 in a fixed order (the loss in double): a row's pairs by waves in turn, waves by number, splits by number.
+// Bound by fetching two rows of labels per pair from anywhere.  A wave takes a chunk of consecutive pairs whatever rows they are of (rows have
+// very unequal numbers of them), four at a time, whole rows of weights in its registers; the difference that makes the margin makes the
+// gradient too, so rows are fetched once.  Where a row's pairs end the wave stores its dX, or, of a row that the chunk has only
+// a part of, that part: preference_finish_kernel adds those up.  Everything is summed in fp32 in a fixed order (the loss in double): pairs in
+// their order within a chunk, chunks in theirs.
 #pragma once
 #include "mx4.hpp"
 
@@ -15,6 +17,7 @@ namespace xfc {
 
 constexpr int PREF_WAVES = 4;
 constexpr int pref_pairs(int pieces) { return pieces <= 2 ? 4 : 8 / pieces; }  // as many as the registers hold
+constexpr int PREF_FINISH = 1024;
 constexpr int PREF_TILE = 512;  // pairs of a row whose entries of G are joined at a time
 
 struct PrefArgs {
@@ -23,13 +26,14 @@ struct PrefArgs {
   int64_t L; int d;
   const int32_t* rowptr; const int32_t* chosen; const int32_t* rejected;
   const float* reference; const float* weight;        // may be null: 0, 1
-  int B, P, splits;
+  int B, P;
+  int chunk, chunks;                                   // pairs of a wave; waves
   float beta, smoothing, scale;
   float* margin;                                       // may be null
   void* dX; int dx_type; int64_t lddx;                 // may be null
   half_t* G; int64_t ldg;                              // may be null
   float* loss;
-  float* slope; double* part_loss; float* part_dx;     // workspace: P; B x splits; B x splits x d with several splits and dX
+  float* slope; double* part_loss; float* part_dx;     // workspace: P; chunks; chunks x 2 x d, the parts of a chunk's first and last row
 };
 
 // Pairs of a row, whatever rowptr holds.
@@ -55,42 +59,68 @@ __device__ __forceinline__ Float8 pref_load(const PrefArgs& a, int label, int k)
   }
 }
 
+// The wave's sum, uniform: within rows of 16 lanes, then across them.
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  auto step = [&](auto ctrl, auto rows) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1, 2, 4, 8
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15, 31
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Eight neighbouring elements of a row of dX.
+__device__ __forceinline__ void pref_store(const PrefArgs& a, int64_t at, const Float8& f) {
+  if (a.dx_type == XFC_F32) store8<XFC_F32>(reinterpret_cast<float*>(a.dX) + at, f);
+  else if (a.dx_type == XFC_BF16) store8<XFC_BF16>(reinterpret_cast<uint16_t*>(a.dX) + at, f);
+  else store8<XFC_F16>(reinterpret_cast<half_t*>(a.dX) + at, f);
 }
 
 // C pieces of 512 dims.
 template <int C, bool MX>
 __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a) {
   constexpr int PAIRS = pref_pairs(C);
-  __shared__ float sums[PREF_WAVES][C * 512];
-  __shared__ double losses[PREF_WAVES];
-  const int row = blockIdx.x, split = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int begin, end;
-  pref_range(a, row, begin, end);
-  const int per = (end - begin + a.splits - 1) / a.splits;
-  const int first = begin + split * per, last = first + per < end ? first + per : end;
-
-  Float8 x[C], acc[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int k = 512 * c + 8 * lane;
-    x[c] = Float8{};
-    acc[c] = Float8{};
-    if (k < a.d) x[c] = load8_of(a.X, a.type, (int64_t)row * a.ldx + k);
+  const int lane = threadIdx.x & 63, chunk = blockIdx.x * PREF_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (chunk >= a.chunks) return;
+  const int p0 = chunk * a.chunk, p1 = p0 + a.chunk < a.P ? p0 + a.chunk : a.P;  // a.chunk <= 64
+  // a pair for each lane
+  const bool in = p0 + lane < p1;
+  const int cl = in ? a.chosen[p0 + lane] : -1, rl = in ? a.rejected[p0 + lane] : -1;
+  const float ref = in && a.reference ? a.reference[p0 + lane] : 0.f, wt = in && a.weight ? a.weight[p0 + lane] : 1.f;
+  // the row of the first pair: the last one that begins at it or before (B: none)
+  int row = 0;
+  for (int left = a.B; left > 0;) {  // 64 of them looked at at a time
+    const int step = (left + 63) / 64, mid = (lane + 1) * step - 1;
+    const int past = __builtin_popcountll(__ballot(mid < left && a.rowptr[row + (mid < left ? mid : 0) + 1] <= p0));
+    row += past * step;
+    left = left - past * step < step - 1 ? left - past * step : step - 1;
   }
+  row = __builtin_amdgcn_readfirstlane(row);
+  const unsigned long long usable = __ballot(cl >= 0 && cl < a.L && rl >= 0 && rl < a.L && wt != 0.f);
+  float my_margin = 0.f, my_slope = 0.f;
   double loss = 0.0;
-  // 64 pairs at a time: their lists by one load each, every fourth of them this wave's
-  for (int p0 = first; p0 < last; p0 += 64 * PREF_WAVES) {
-    const int p = p0 + lane * PREF_WAVES + wave;
-    const bool in = p < last;
-    const int cl = in ? a.chosen[p] : -1, rl = in ? a.rejected[p] : -1;
-    const float ref = in && a.reference ? a.reference[p] : 0.f, wt = in && a.weight ? a.weight[p] : 1.f;
-    unsigned long long left = __ballot(cl >= 0 && cl < a.L && rl >= 0 && rl < a.L && wt != 0.f);
-    float my_margin = 0.f, my_slope = 0.f;
+  for (int p = p0; p < p1 && row < a.B; ++row) {
+    int begin, end;
+    pref_range(a, row, begin, end);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    const int first = p > begin ? p : begin, last = end < p1 ? end : p1;  // of the row, in this chunk
+    if (first >= last) continue;
+    unsigned long long left = usable & (~0ull << (first - p0)) & (~0ull >> (64 - (last - p0)));
+    Float8 acc[C];
+    Float8 x[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int k = 512 * c + 8 * lane;
+      acc[c] = Float8{};
+      x[c] = Float8{};
+      if (k < a.d) x[c] = load8_of(a.X, a.type, (int64_t)row * a.ldx + k);
+    }
     while (left) {
       int at[PAIRS], n = 0;
 #pragma unroll
@@ -124,7 +154,8 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         if (j < n) {
-          const float m = z[j] - __shfl(ref, at[j], 64), t = a.beta * m, w = __shfl(wt, at[j], 64);
+          const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), at[j]));
+          const float m = z[j] - __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ref), at[j])), t = a.beta * m;
           const float small = expf(-fabsf(t)), sig = t >= 0.f ? 1.f / (1.f + small) : small / (1.f + small);
           // (a positive margin's slope is -(1 - sigmoid) + e: formed so, what is left at sigmoid near 1 keeps its bits)
           const float g = w * a.beta * (t >= 0.f ? a.smoothing - small / (1.f + small) : sig - (1.f - a.smoothing));
@@ -137,86 +168,79 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
         }
       }
     }
-    if (in) {
-      if (a.margin) a.margin[p] = my_margin;
-      if (a.G) a.slope[p] = my_slope;
-    }
-  }
-  if (a.margin && split == 0) {  // pairs that no row has
-    if (row == 0)
-      for (int p = tid; p < a.P && p < begin; p += 64 * PREF_WAVES) a.margin[p] = 0.f;
-    if (row == a.B - 1)
-      for (int p = end + tid; p < a.P; p += 64 * PREF_WAVES) a.margin[p] = 0.f;
-  }
-  if (lane == 0) losses[wave] = loss;
-  if (a.dX) {
+    if (a.dX) {
+      const bool whole = begin >= p0 && end <= p1;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
+        const int k = 512 * c + 8 * lane;
+        if (k >= a.d) continue;
+        if (whole) {
 #pragma unroll
-      for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<float4v*>(&sums[wave][512 * c + 8 * lane + e]) = float4v{acc[c].v[e], acc[c].v[e + 1], acc[c].v[e + 2], acc[c].v[e + 3]};
-  }
-  __syncthreads();
-  if (tid == 0) {
-    double t = 0.0;
-    for (int w = 0; w < PREF_WAVES; ++w) t += losses[w];
-    a.part_loss[(int64_t)row * a.splits + split] = t;
-  }
-  if (a.dX) {
-    for (int k = tid; k < a.d; k += 64 * PREF_WAVES) {
-      float t = 0.f;
-      for (int w = 0; w < PREF_WAVES; ++w) t += sums[w][k];
-      if (a.splits > 1) {
-        a.part_dx[((int64_t)row * a.splits + split) * a.d + k] = t;
-      } else {
-        t *= a.scale;
-        const int64_t to = (int64_t)row * a.lddx + k;
-        if (a.dx_type == XFC_F32) reinterpret_cast<float*>(a.dX)[to] = t;
-        else if (a.dx_type == XFC_BF16) reinterpret_cast<__bf16*>(a.dX)[to] = (__bf16)t;
-        else reinterpret_cast<half_t*>(a.dX)[to] = (half_t)t;
+          for (int e = 0; e < 8; ++e) acc[c].v[e] *= a.scale;
+          pref_store(a, (int64_t)row * a.lddx + k, acc[c]);
+        } else {
+          float* const to = a.part_dx + (2 * (int64_t)chunk + (begin >= p0 ? 1 : 0)) * a.d + k;
+          store8<XFC_F32>(to, acc[c]);
+        }
       }
     }
+    p = last;
   }
+  if (in) {
+    if (a.margin) a.margin[p0 + lane] = my_margin;
+    if (a.G) a.slope[p0 + lane] = my_slope;
+  }
+  if (lane == 0) a.part_loss[chunk] = loss;
 }
 
-// What is left after the pairs, a workgroup per row: the sum of the splits' dX, and G.  A row's entries of G, two a pair, are
-// joined PREF_TILE pairs at a time: each is compared with all others, the first of a label adds up all of them in their order and
-// rounds G once.  Workgroup B sums the loss.
-__global__ void __launch_bounds__(256) preference_finish_kernel(PrefArgs a) {
-  __shared__ int32_t label[2 * PREF_TILE];
-  __shared__ float slope[2 * PREF_TILE];
-  __shared__ double sums[4];
+// What is left after the pairs, a workgroup per row: dX of rows without pairs and of those that several chunks have a part of, and G.
+// A row's entries of G, two a pair, are joined PREF_TILE pairs at a time: each is compared with all others, the first of a label adds up all of them, in an order that
+// their number alone decides, and rounds G once.  Workgroup B sums the loss.
+__global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs a) {
+  __shared__ __attribute__((aligned(16))) int32_t label[2 * PREF_TILE];
+  __shared__ __attribute__((aligned(16))) float slope[2 * PREF_TILE];
+  __shared__ double sums[PREF_FINISH / 64];
   const int row = blockIdx.x, tid = threadIdx.x;
   if (row == (int)gridDim.x - 1) {
     double t = 0.0;
-    for (int64_t i = tid; i < (int64_t)a.B * a.splits; i += 256) t += a.part_loss[i];
+    for (int i = tid; i < a.chunks; i += PREF_FINISH) t += a.part_loss[i];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
     if ((tid & 63) == 0) sums[tid >> 6] = t;
     __syncthreads();
-    if (tid == 0) *a.loss = (float)(((sums[0] + sums[1]) + sums[2]) + sums[3]);
+    if (tid == 0) {
+      for (int w = 1; w < PREF_FINISH / 64; ++w) t += sums[w];
+      *a.loss = (float)t;
+    }
     return;
   }
-  if (a.dX && a.splits > 1) {
-    for (int k = tid; k < a.d; k += 256) {
-      float t = 0.f;
-      for (int s = 0; s < a.splits; ++s) t += a.part_dx[((int64_t)row * a.splits + s) * a.d + k];
-      t *= a.scale;
-      const int64_t to = (int64_t)row * a.lddx + k;
-      if (a.dx_type == XFC_F32) reinterpret_cast<float*>(a.dX)[to] = t;
-      else if (a.dx_type == XFC_BF16) reinterpret_cast<__bf16*>(a.dX)[to] = (__bf16)t;
-      else reinterpret_cast<half_t*>(a.dX)[to] = (half_t)t;
+  int begin, end;
+  pref_range(a, row, begin, end);
+  if (a.dX) {
+    const int first = begin / a.chunk, last = end > begin ? (end - 1) / a.chunk : first;
+    if (begin == end || first < last) {
+      for (int k = 8 * tid; k < a.d; k += 8 * PREF_FINISH) {
+        Float8 t = {};
+        if (begin < end) {
+          for (int c = first; c <= last; ++c) {
+            const Float8 part = load8<XFC_F32>(a.part_dx + (2 * (int64_t)c + (c == first ? 1 : 0)) * a.d + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t.v[e] += part.v[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t.v[e] *= a.scale;
+        pref_store(a, (int64_t)row * a.lddx + k, t);
+      }
     }
   }
   if (!a.G) return;
-  int begin, end;
-  pref_range(a, row, begin, end);
   half_t* const g = a.G + (int64_t)row * a.ldg;
   for (int p0 = begin; p0 < end; p0 += PREF_TILE) {
-    const int n = end - p0 < PREF_TILE ? end - p0 : PREF_TILE;
+    const int n = end - p0 < PREF_TILE ? end - p0 : PREF_TILE, quads = (n + 1) / 2;
     __syncthreads();
-    for (int e = tid; e < n; e += 256) {
-      const int c = a.chosen[p0 + e], r = a.rejected[p0 + e];
+    for (int e = tid; e < 2 * quads; e += PREF_FINISH) {  // an odd number of pairs is filled up with one that is none
+      const int c = e < n ? a.chosen[p0 + e] : -1, r = e < n ? a.rejected[p0 + e] : -1;
       const bool ok = c >= 0 && c < a.L && r >= 0 && r < a.L && (!a.weight || a.weight[p0 + e] != 0.f);
       const float s = ok ? a.slope[p0 + e] : 0.f;
       label[2 * e] = ok ? c : -1;
@@ -225,16 +249,27 @@ __global__ void __launch_bounds__(256) preference_finish_kernel(PrefArgs a) {
       slope[2 * e + 1] = -s;
     }
     __syncthreads();
-    for (int e = tid; e < 2 * n; e += 256) {
+    for (int e = tid >> 2; e < 2 * n; e += PREF_FINISH / 4) {  // four neighbouring lanes an entry, every fourth quad each
       const int mine = label[e];
       float t = 0.f;
-      bool owner = mine >= 0;
-      for (int o = 0; o < 2 * n; ++o) {
-        const bool same = label[o] == mine;
-        owner = owner && !(same && o < e);
-        t += same ? slope[o] : 0.f;
+      int first = e;
+#pragma unroll 4
+      for (int o = tid & 3; o < quads; o += 4) {
+        const int4v l = reinterpret_cast<const int4v*>(label)[o];
+        const float4v s = reinterpret_cast<const float4v*>(slope)[o];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          first = l[j] == mine && 4 * o + j < first ? 4 * o + j : first;
+          t += l[j] == mine ? s[j] : 0.f;
+        }
       }
-      if (owner) g[mine] = (half_t)((float)g[mine] + t);
+#pragma unroll
+      for (int off = 1; off < 4; off <<= 1) {
+        t += __shfl_xor(t, off, 64);
+        const int other = __shfl_xor(first, off, 64);
+        first = other < first ? other : first;
+      }
+      if ((tid & 3) == 0 && first == e && mine >= 0) g[mine] = (half_t)((float)g[mine] + t);
     }
   }
 }

@@ -83,8 +83,6 @@ def preference(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.
     loss = torch.empty((), dtype=torch.float32, device=device)
     margin = torch.empty(P, dtype=torch.float32, device=device) if need_margin else None
     grad = torch.empty(bsz, dims, dtype=grad_dtype, device=device) if g is None and need_grad else None
-    if bsz == 0 and need_margin:
-        margin.zero_()
     L = lib()
     need = L.xfc_preference_workspace_bytes(bsz, P, dims)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
