@@ -310,9 +310,11 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
                    int64_t B, int64_t L, int64_t d, int embed_bits, void* stream);
 
 /*
- * xfc_topk with an MX4 label matrix, with the same order of ties, places without a score and clamp to numy.  K <= 8: by the fp32 sums, no logits
- * are written; 8 < K <= 8192: by the logits of xfc_mx4_logits.  Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, K); with
- * K > 8 and more than 256 rows what 256 rows take is enough, the rows then go in turns.
+ * xfc_topk with an MX4 label matrix: ties to the lower label, labels >= numy returned as numy - 1.  K <= 8: by the fp32 sums; a score that is no number is
+ * never selected, and a row with fewer than K others reports (-inf, numy - 1) in the remaining places.  8 < K <= 8192: by the logits of
+ * xfc_mx4_logits, a NaN as -inf.  Up to K = 256 of 4096 K labels or more no logits are written either, only maxima of blocks of labels.
+ * Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, K); where logits are written and there are more than 256 rows, what 256
+ * rows take is enough, the rows then go in turns.
  */
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K);
 int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,

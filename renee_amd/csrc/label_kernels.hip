@@ -90,10 +90,12 @@ int launch_product(const MxPlan& p, const MxProductArgs& a, hipStream_t st) {
 }
 int launch_product(int out, bool x8, const MxPlan& p, const MxProductArgs& a, hipStream_t st) {
   if (x8) {
+    if (out == MX_HALF_MAXIMA) return launch_product<true, MX_HALF_MAXIMA>(p, a, st);
     if (out == MX_LOGITS) return launch_product<true, MX_LOGITS>(p, a, st);
     if (out == MX_LOGITS_MAX) return launch_product<true, MX_LOGITS_MAX>(p, a, st);
     return launch_product<true, MX_MAXIMA>(p, a, st);
   }
+  if (out == MX_HALF_MAXIMA) return launch_product<false, MX_HALF_MAXIMA>(p, a, st);
   if (out == MX_LOGITS) return launch_product<false, MX_LOGITS>(p, a, st);
   if (out == MX_LOGITS_MAX) return launch_product<false, MX_LOGITS_MAX>(p, a, st);
   return launch_product<false, MX_MAXIMA>(p, a, st);
@@ -137,6 +139,10 @@ int check_product(const void* X, int type, int64_t ldx, const void* codes, const
 int64_t mx_half_maxima(int64_t L) { return 2 * (int64_t)ceil_div(L, MX_UNIT); }
 int64_t mx_maxima(int64_t L) { return round_up(ceil_div(L, MX_UNIT), 4); }
 
+// What mx4_select_kernel takes at most: its own, and the row's numbers at 16,384 dims (8 bits: 9,088).
+constexpr int MX_SELECT_LDS = 96 * 1024;
+static_assert(sizeof(MxSelectLds) + 128 * MxScores<false>::STEP_BYTES <= MX_SELECT_LDS && sizeof(MxSelectLds) + 71 * MxScores<true>::STEP_BYTES <= MX_SELECT_LDS, "LDS budget");
+
 }  // namespace
 
 int xfc::init_labels() {
@@ -154,6 +160,9 @@ int xfc::init_labels() {
   both(std::integral_constant<int, MX_LOGITS>{});
   both(std::integral_constant<int, MX_LOGITS_MAX>{});
   both(std::integral_constant<int, MX_MAXIMA>{});
+  both(std::integral_constant<int, MX_HALF_MAXIMA>{});
+  keep(raise_lds_limit<mx4_select_kernel<true>>(MX_SELECT_LDS));
+  keep(raise_lds_limit<mx4_select_kernel<false>>(MX_SELECT_LDS));
   return e == hipSuccess ? XFC_OK : XFC_ERR_HIP;
 }
 
@@ -197,7 +206,9 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
                     reinterpret_cast<hipStream_t>(stream));
 }
 
-// K > 8: the logits of this many rows, and the maxima of their blocks
+// K > 8: by logits, or by maxima of 32 labels and the K best blocks' scores formed again.
+static bool mx_by_maxima(int64_t L, int64_t K) { return K <= MX_SELECT_K && L >= 4096 * K; }
+// By logits: those of this many rows, and the maxima of their blocks
 static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
   const size_t logits = (size_t)rows * (size_t)round_up(L, 8) * 2;
   return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_half_maxima(L) * 2 : 0);
@@ -205,7 +216,7 @@ static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
 
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K) {
   if (!dims_ok(B) || !dims_ok(L) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
-  if (K <= TOPK_MAX) return (size_t)B * (size_t)mx_maxima(L) * 4;
+  if (K <= TOPK_MAX || mx_by_maxima(L, K)) return (size_t)B * (size_t)mx_maxima(L) * 4;
   return mx_logit_rows_bytes(B, L, K);
 }
 
@@ -214,12 +225,13 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   int rc = check_product(X, type, ldx, codes, scales, B, L, d, embed_bits);
   if (rc || B == 0) return rc;
   if (K < 1 || K > SEL_MAX_K || L < K || numy < 1 || !values || !indices) return XFC_ERR_INVALID;
-  const int64_t least = B < 256 || K <= TOPK_MAX ? B : 256;
+  const bool maxima = K <= TOPK_MAX || mx_by_maxima(L, K);
+  const int64_t least = B < 256 || maxima ? B : 256;
   if (!workspace || workspace_bytes < xfc_mx4_topk_workspace_bytes(least, L, K)) return XFC_ERR_WORKSPACE;
   if (!aligned16(workspace)) return XFC_ERR_ALIGN;
   const bool x8 = embed_bits == 8;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (K > TOPK_MAX) {
+  if (!maxima) {
     const int64_t ldb = mx_half_maxima(L);
     int64_t block = B;
     if (workspace_bytes < xfc_mx4_topk_workspace_bytes(B, L, K)) block = (int64_t)(workspace_bytes / xfc_mx4_topk_workspace_bytes(256, L, K)) * 256;
@@ -228,7 +240,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
       const int64_t rows = B - r0 < block ? B - r0 : block;
       half_t* const logits = (half_t*)workspace;
       half_t* const hmax = select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? logits + round_up(rows * ldl, 8) : nullptr;
-      rc = mx_product(hmax ? MX_LOGITS_MAX : MX_LOGITS, x8, reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type), type, ldx, codes, scales,
+      rc = mx_product(MX_LOGITS_MAX, x8, reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type), type, ldx, codes, scales,
                       logits, ldl, hmax, nullptr, ldb, rows, L, d, 1, st);
       if (rc) return rc;
       rc = select_rows(logits, ldl, (int)rows, (int)L, numy, K, hmax, ldb, values + r0 * K, indices + r0 * K, st);
@@ -238,13 +250,19 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   }
   float* const bmax = (float*)workspace;
   const int64_t ldb = mx_maxima(L);
-  rc = mx_product(MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d, L >= (1 << 20) ? 4 : 1, st);
+  rc = mx_product(K > TOPK_MAX ? MX_HALF_MAXIMA : MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d, L >= (1 << 20) ? 4 : 1, st);
   if (rc) return rc;
   PickArgs k = {};
-  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, MX_UNIT); k.N = (int)L; k.K = (int)d; k.topk = K;
+  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, K > TOPK_MAX ? 32 : MX_UNIT); k.N = (int)L; k.K = (int)d; k.topk = K;
   k.begin = k.end = 1; k.numy = numy; k.out_v = values; k.out_i = indices;
   auto pick = [&](auto s) {
     using S = decltype(s);
+    if (K > TOPK_MAX) {
+      constexpr auto kernel = mx4_select_kernel<std::is_same_v<S, MxScores<true>>>;
+      if (raise_lds_limit<kernel>(MX_SELECT_LDS) != hipSuccess) return (int)XFC_ERR_HIP;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)B), dim3(MX_SELECT_THREADS), (unsigned)(S::lds(d) + sizeof(MxSelectLds)), st, k, s);
+      return check_launch();
+    }
     hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 18 KB at most
     return check_launch();
   };

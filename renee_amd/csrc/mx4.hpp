@@ -277,13 +277,15 @@ __device__ __forceinline__ const XFC_GLB uint8_t* scalar(const uint8_t* p) {
   return g;
 }
 
-enum MxOut { MX_LOGITS, MX_LOGITS_MAX, MX_MAXIMA };
+// MX_LOGITS: logits.  MX_LOGITS_MAX: the same for a selection, numbers only (a NaN becomes -inf), with the largest of every 32.
+// MX_MAXIMA: the largest sum of every unit.  MX_HALF_MAXIMA: the largest of every 32 as a logit, no number counts as -inf.
+enum MxOut { MX_LOGITS, MX_LOGITS_MAX, MX_MAXIMA, MX_HALF_MAXIMA };
 
 struct MxProductArgs {
   const void* X; int type; int64_t ldx;  // M rows of K
   const uint8_t* codes; const uint8_t* scales;
   half_t* out; int64_t ldo;              // logits
-  half_t* hmax; float* bmax; int64_t ldb; // maxima: of the logits as stored of 32 labels, of the sums of a unit
+  half_t* hmax; float* bmax; int64_t ldb; // beside logits; alone: a float or two halves for a unit
   int M, N, K;
   int units, blocks, steps;
   int tiles_m, slots;                    // row tiles; workgroups of a row tile on an XCD
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     const int i = lane_now & 15, q = lane_now >> 4;
     const int label0 = unit * MX_UNIT;
     const bool edge = label0 + MX_UNIT > a.N;
-    if constexpr (OUT == MX_MAXIMA) {
+    if constexpr (OUT == MX_MAXIMA || OUT == MX_HALF_MAXIMA) {
       // The maxima below are inline asm, in front of which the compiler puts no wait states: the last MFMAs' results are waited for here.
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_nop 15\n\ts_nop 15");
@@ -401,18 +403,26 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
             for (int j = 0; j < NT; ++j) acc[t][j][r] = in ? acc[t][j][r] : __builtin_nanf("");
           }
       }
-      auto largest = [&](int j) {  // of this lane's sixteen labels
-        j = j < NT ? j : NT - 1;
-        float m = acc[0][j][0];
-#pragma unroll
-        for (int e = 1; e < 15; e += 2) m = max3_num(m, acc[e >> 2][j][e & 3], acc[(e + 1) >> 2][j][(e + 1) & 3]);
-        return max_num(m, acc[3][j][3]);
+      // of this lane's eight labels of half p
+      auto largest = [&](int j, int p) {
+        const float4v lo = acc[2 * p][j < NT ? j : NT - 1], hi = acc[2 * p + 1][j < NT ? j : NT - 1];
+        return max3_num(max3_num(lo[0], lo[1], lo[2]), lo[3], max3_num(hi[0], hi[1], max_num(hi[2], hi[3])));
       };
+      // lane group g ends up with row tile 4 n + g
+      auto over_lanes = [&](int n, auto of) { return fold16(fold32(of(4 * n), of(4 * n + 2)), fold32(of(4 * n + 1), of(4 * n + 3))); };
       const int r4 = unit & (run - 1);
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
-        // lane group g ends up with row tile 4 n + g
-        const float m = fold16(fold32(largest(4 * n), largest(4 * n + 2)), fold32(largest(4 * n + 1), largest(4 * n + 3)));
+        float m;
+        if constexpr (OUT == MX_MAXIMA) {
+          m = over_lanes(n, [&](int j) { return max_num(largest(j, 0), largest(j, 1)); });
+        } else {
+          typedef half_t half2v __attribute__((ext_vector_type(2)));
+          const float least = -__builtin_huge_valf();
+          const half2v two = {(half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 0); }), least),
+                              (half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 1); }), least)};
+          m = __builtin_bit_cast(float, two);
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) best[n][r] = r4 == r ? m : best[n][r];
       }
@@ -437,6 +447,10 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
           half8 h;
 #pragma unroll
           for (int r = 0; r < 4; ++r) { h[r] = (half_t)acc[2 * p][j][r]; h[4 + r] = (half_t)acc[2 * p + 1][j][r]; }
+          if constexpr (OUT == MX_LOGITS_MAX) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = h[e] == h[e] ? h[e] : (half_t)-__builtin_huge_valf();
+          }
           const int col = label0 + 32 * p + 8 * q;
           if constexpr (OUT == MX_LOGITS_MAX) {
             half8 m = h;
@@ -458,7 +472,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
         if constexpr (OUT == MX_LOGITS_MAX) {
           const uint32_t v = pk_fold32(largest[0], largest[1]);
           const half_t m = pk_larger(pk_fold16(v, v));
-          if (row < a.M && (q & 1) == 0) a.hmax[(int64_t)row * a.ldb + 2 * (int64_t)unit + (q >> 1)] = m;
+          if (a.hmax && row < a.M && (q & 1) == 0) a.hmax[(int64_t)row * a.ldb + 2 * (int64_t)unit + (q >> 1)] = m;
         }
       }
     }
@@ -493,7 +507,7 @@ struct MxScores {
   }
   // bytes of a step: block q's numbers behind each other, then four scale bytes
   static constexpr int STEP_BYTES = (X8 ? 128 : 64) + 16;
-  static int64_t lds(int64_t d) { return (int64_t)mx_steps(d) * STEP_BYTES; }
+  __host__ __device__ static int64_t lds(int64_t d) { return (int64_t)mx_steps(d) * STEP_BYTES; }
 
   __device__ __forceinline__ void open(const PickArgs& a, int row) const {
     unsigned char* const at = room();
@@ -535,5 +549,171 @@ struct MxScores {
     return z;
   }
 };
+
+// ---------------------------------------------------------------------------------------------
+// 8 < K <= MX_SELECT_K without logits: the K best blocks of 32 by their maxima, their scores formed again
+// ---------------------------------------------------------------------------------------------
+// Why that is exact: as in topk.hpp, with scores rounded to fp16; the K-th best maximum is no larger than the K-th best score, so
+// that of the K blocks' scores only those that reach it are put in order.
+//
+// One workgroup per row.  The maxima's keys are counted by their upper eleven bits, then those of the bin that the K-th is in by
+// the lower five; blocks above the K-th key are taken, and of those at it the first ones.  Sixteen waves then form the scores as MxScores
+// does, a tile of a block each.  Bound by fetching K x 32 labels a row.
+constexpr int MX_SELECT_K = 256, MX_SELECT_THREADS = 1024, MX_SELECT_BINS = 2048;
+
+// (of PickArgs: bmax, two halves a float; n_blocks of 32 labels; N, K, topk, numy, out_v, out_i)
+struct MxSelectLds {
+  unsigned long long cand[MX_SELECT_K * 32];
+  int hist[MX_SELECT_BINS];
+  int block[MX_SELECT_K];
+  int wave_tot[MX_SELECT_THREADS / 64];
+  int bin, above, n_block, n_cand;
+};
+
+// fp16 bits as a key that orders like the value, -0 as +0, and back.
+__device__ __forceinline__ uint32_t half_key(uint32_t h) {
+  if (h == 0x8000u) h = 0u;
+  return (h & 0x8000u) ? (~h & 0xffffu) : (h | 0x8000u);
+}
+__device__ __forceinline__ float half_unkey(uint32_t k) {
+  const uint16_t h = (uint16_t)((k & 0x8000u) ? (k & 0x7fffu) : ~k);
+  return (float)__builtin_bit_cast(half_t, h);
+}
+
+template <bool X8>
+__global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs a, MxScores<X8> scores) {
+  MxSelectLds& S = *reinterpret_cast<MxSelectLds*>(MxScores<X8>::room() + MxScores<X8>::lds(a.K));  // a multiple of 16
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int K = a.topk < a.n_blocks ? a.topk : a.n_blocks;  // blocks wanted
+  const uint32_t* const maxima = reinterpret_cast<const uint32_t*>(a.bmax) + (int64_t)row * a.ldb;  // two blocks each
+  const int quads = (a.n_blocks + 7) / 8;
+  auto for_each = [&](auto&& f) {
+    for (int w = tid; w < quads; w += MX_SELECT_THREADS) {
+      const uint4v v = *reinterpret_cast<const uint4v*>(maxima + 4 * w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t h = (v[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+        if (8 * w + e < a.n_blocks) f(half_key(h), 8 * w + e);
+      }
+    }
+  };
+  // The bin of the K-th, counted down from the last; above: how many lie in higher ones.  Wave 0.
+  auto find_bin = [&](int bins, int base) {
+    if (wave == 0) {
+      const int per = bins / 64;
+      int mine = 0;
+      for (int j = 0; j < per; ++j) mine += S.hist[lane * per + j];
+      int from = mine;  // of this lane's bins and all higher ones
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_down(from, off, 64);
+        if (lane + off < 64) from += v;
+      }
+      const unsigned long long reach = __ballot(base + from >= K);
+      if (lane == 63 - __builtin_clzll(reach | 1ull)) {
+        int above = base + from - mine, b = lane * per + per - 1;
+        for (; b > lane * per; --b) {
+          if (above + S.hist[b] >= K) break;
+          above += S.hist[b];
+        }
+        S.bin = b;
+        S.above = above;
+      }
+    }
+    __syncthreads();
+  };
+  for (int i = tid; i < MX_SELECT_BINS; i += MX_SELECT_THREADS) S.hist[i] = 0;
+  if (tid == 0) S.n_block = S.n_cand = 0;
+  scores.open(a, row);
+  __syncthreads();
+  for_each([&](uint32_t key, int) { atomicAdd(&S.hist[key >> 5], 1); });
+  __syncthreads();
+  find_bin(MX_SELECT_BINS, 0);
+  const int top = S.bin, above = S.above;
+  __syncthreads();
+  if (tid < 64) S.hist[tid] = 0;
+  __syncthreads();
+  for_each([&](uint32_t key, int) { if ((int)(key >> 5) == top) atomicAdd(&S.hist[key & 31], 1); });
+  __syncthreads();
+  find_bin(64, above);
+  const uint32_t least = (uint32_t)top * 32 + (uint32_t)S.bin;
+  const int at_least = K - S.above;  // blocks at the K-th key that are taken, the first ones
+  // (the list's order is of no matter)
+  int taken = 0;
+  for (int w0 = 0; w0 < quads; w0 += MX_SELECT_THREADS) {
+    uint32_t here = 0, equal = 0;  // of this thread's eight blocks: above the key, at it
+    if (w0 + tid < quads) {
+      const uint4v v = *reinterpret_cast<const uint4v*>(maxima + 4 * (w0 + tid));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = half_key((v[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+        if (8 * (w0 + tid) + e < a.n_blocks) {
+          here |= (key > least ? 1u : 0u) << e;
+          equal |= (key == least ? 1u : 0u) << e;
+        }
+      }
+    }
+    // the equal ones' ranks, in the order of blocks
+    int mine = __builtin_popcount(equal), rank = mine;
+    const bool any = __syncthreads_or(mine != 0 && taken < at_least);
+    if (any) {
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(rank, off, 64);
+        if (lane >= off) rank += v;
+      }
+      if (lane == 63) S.wave_tot[wave] = rank;
+      __syncthreads();
+      int before = taken, all = 0;
+      for (int w = 0; w < MX_SELECT_THREADS / 64; ++w) {
+        before += w < wave ? S.wave_tot[w] : 0;
+        all += S.wave_tot[w];
+      }
+      before += rank - mine;
+      for (uint32_t left = equal; left && before < at_least; left &= left - 1, ++before) here |= left & (0u - left);
+      taken += all;
+    }
+    for (; here; here &= here - 1) S.block[atomicAdd(&S.n_block, 1)] = 8 * (w0 + tid) + __builtin_ctz(here);
+    __syncthreads();
+  }
+  const int n_block = S.n_block;  // K
+  for (int u = wave; u < 2 * n_block; u += MX_SELECT_THREADS / 64) {
+    const int first = S.block[u >> 1] * 32, part = 2 * ((first / 32) & 1) + (u & 1);
+    const float4v z = scores.score(a, row, first & ~(MX_UNIT - 1), part, lane);
+    if ((lane & 15) == 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int label = (first & ~(MX_UNIT - 1)) + mx_label(part, 4 * (lane >> 4) + r);
+        const half_t h = z[r] == z[r] ? (half_t)z[r] : (half_t)-__builtin_huge_valf();
+        const uint32_t key = half_key(__builtin_bit_cast(uint16_t, h));
+        if (label < a.N && (key >= least || n_block < a.topk)) S.cand[atomicAdd(&S.n_cand, 1)] = ((unsigned long long)key << 32) | (uint32_t)~label;
+      }
+    }
+  }
+  __syncthreads();
+  // in order: bitonic over the next power of two
+  const int n = S.n_cand;
+  int size = 64;
+  while (size < n) size <<= 1;
+  for (int i = n + tid; i < size; i += MX_SELECT_THREADS) S.cand[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = tid; i < size; i += MX_SELECT_THREADS) {
+        const int o = i ^ j;
+        if (o > i) {
+          const unsigned long long x = S.cand[i], y = S.cand[o];
+          if ((x < y) == ((i & k) == 0)) { S.cand[i] = y; S.cand[o] = x; }
+        }
+      }
+      __syncthreads();
+    }
+  for (int i = tid; i < a.topk; i += MX_SELECT_THREADS) {
+    const unsigned long long c = S.cand[i];
+    const int64_t label = (int64_t)(uint32_t)~(uint32_t)c;
+    a.out_v[(int64_t)row * a.topk + i] = half_unkey((uint32_t)(c >> 32));
+    a.out_i[(int64_t)row * a.topk + i] = label < a.numy ? label : a.numy - 1;
+  }
+}
 
 }  // namespace xfc

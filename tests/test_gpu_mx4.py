@@ -131,7 +131,9 @@ def test_topk_with_4_bits(dev, B, L, d, K):
     assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
 
 
-@pytest.mark.parametrize("B,L,d,K", [(2, 70001, 64, 5), (40, 66000, 128, 100), (5, 140003, 64, 8), (3, 70001, 64, 3000)])
+# (above 8 by maxima alone from 4096 K labels on)
+@pytest.mark.parametrize("B,L,d,K", [(2, 70001, 64, 5), (40, 66000, 128, 100), (5, 140003, 64, 8), (3, 70001, 64, 3000), (1, 36864, 8, 9), (130, 40961, 72, 10),
+                                     (33, 70001, 200, 16), (3, 414001, 64, 100), (2, 1050003, 32, 256)])
 def test_topk_of_many_labels(dev, B, L, d, K):
     x, w, z = _problem(B, L, d, 4, torch.float16, L + K)
     v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=4)
@@ -164,6 +166,25 @@ def test_topk_ties_go_to_the_lower_label_and_constant_rows(dev):
             v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=bits)
             ev, ei = O.topk((x.double() @ w.double().t()), K)
             assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
+
+
+@pytest.mark.parametrize("K", [9, 12])
+@pytest.mark.parametrize("L", [1000, 50003])
+def test_topk_above_8_counts_nan_as_the_least(dev, L, K):
+    """Rows of equal scores, of fewer numbers than K, of none, and of infinities."""
+    w = torch.zeros(L, 64, dtype=torch.float16)
+    w[:, 0] = torch.randint(-2, 3, (L,), generator=torch.Generator().manual_seed(L)).half()
+    w[5::3] = float("nan")
+    w[:, 40] = torch.where(torch.arange(L) % 1009 == 7, 6.0e4, 0.0).half()
+    x = torch.zeros(5, 64, dtype=torch.float32)
+    x[0, 0], x[1, 1], x[2, 0], x[3, 40], x[4, 40] = 1.0, 1.0, float("nan"), 1e30, -1e30
+    some = w.clone()
+    some[4:] = float("nan")
+    for m in (w, some):
+        z = (O.rounded(x, 4) @ O.rounded(m, 4).t()).half().double()
+        ev, ei = O.topk(torch.where(torch.isnan(z), -math.inf, z), K)
+        v, i = MX4Labels.from_weight(m.to(dev)).topk(x.to(dev), K, numy=L - 1, embed_bits=4)
+        assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei.clamp(max=L - 2))
 
 
 def test_topk_without_scores_and_clamped_labels(dev):
