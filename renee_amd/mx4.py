@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .xfc import _require, _round_up
+from .xfc import _require, g_row_stride
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # xfc_type
 
@@ -123,7 +123,7 @@ class MX4Labels:
         """Logits embed . W^T in float16 (dl_base.py:568-573), into `out` if it is given."""
         x = _rows(embed, self.device, self.dims, "embed")
         _require(embed_bits in (4, 8), "embed_bits must be 4 or 8", ValueError)
-        bsz, ld = x.shape[0], _round_up(self.numy, 8)
+        bsz, ld = x.shape[0], g_row_stride(self.numy)
         if out is None:
             out = torch.empty(bsz, ld, dtype=torch.float16, device=self.device)
             if ld != self.numy:
