@@ -106,7 +106,7 @@ constexpr int64_t MX_ROWS = 2048;
 
 // All rows of a product, in as many launches as it takes.
 int mx_product(int out, bool x8, const void* X, int type, int64_t ldx, const void* codes, const void* scales, half_t* logits, int64_t ldo,
-               half_t* hmax, float* bmax, int64_t ldb, int64_t B, int64_t L, int64_t d, int run, hipStream_t st) {
+               half_t* hmax, float* bmax, int64_t ldb, int64_t B, int64_t L, int64_t d, int run, bool fine, hipStream_t st) {
   for (int64_t r0 = 0; r0 < B; r0 += MX_ROWS) {
     const int64_t rows = B - r0 < MX_ROWS ? B - r0 : MX_ROWS;
     const MxPlan p = mx_plan(rows, L, d, x8, run, num_cus());
@@ -118,7 +118,7 @@ int mx_product(int out, bool x8, const void* X, int type, int64_t ldx, const voi
     a.hmax = hmax ? hmax + r0 * ldb : nullptr; a.bmax = bmax ? bmax + r0 * ldb : nullptr; a.ldb = ldb;
     a.M = (int)rows; a.N = (int)L; a.K = (int)d;
     a.units = ceil_div(L, MX_UNIT); a.blocks = mx_blocks(d); a.steps = mx_steps(d);
-    a.tiles_m = p.tiles_m; a.slots = p.slots; a.run = run;
+    a.tiles_m = p.tiles_m; a.slots = p.slots; a.run = run; a.fine = fine;
     const int rc = launch_product(out, x8, p, a, st);
     if (rc) return rc;
   }
@@ -135,9 +135,15 @@ int check_product(const void* X, int type, int64_t ldx, const void* codes, const
   return XFC_OK;
 }
 
-// maxima of a row: of 32 logits, of the units' sums, whole runs of them
-int64_t mx_half_maxima(int64_t L) { return 2 * (int64_t)ceil_div(L, MX_UNIT); }
-int64_t mx_maxima(int64_t L) { return round_up(ceil_div(L, MX_UNIT), 4); }
+// Maxima of a row, as floats.  Up to MX_FINE_ROWS rows a float for each half of a unit, else for each unit, and for K > 8 two halves in its place;
+// whole runs of units, whole pieces of 16 bytes.
+constexpr int64_t MX_FINE_ROWS = 32;
+bool mx_fine(int64_t B, int64_t K) { return K <= TOPK_MAX && B <= MX_FINE_ROWS; }
+int64_t mx_maxima(int64_t B, int64_t L, int64_t K) {
+  const int64_t units = ceil_div(L, MX_UNIT);
+  return round_up(mx_fine(B, K) ? 2 * units : units, 4);
+}
+int64_t mx_half_maxima(int64_t L) { return 2 * (int64_t)ceil_div(L, MX_UNIT); }  // beside logits, halves
 
 // What mx4_select_kernel takes at most: its own, and the row's numbers at 16,384 dims (8 bits: 9,088).
 constexpr int MX_SELECT_LDS = 96 * 1024;
@@ -202,7 +208,7 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
   if (!out) return XFC_ERR_INVALID;
   if (ldo % 8 || !aligned16(out)) return XFC_ERR_ALIGN;
   if (ldo < L) return XFC_ERR_SHAPE;
-  return mx_product(MX_LOGITS, embed_bits == 8, X, type, ldx, codes, scales, (half_t*)out, ldo, nullptr, nullptr, 0, B, L, d, 1,
+  return mx_product(MX_LOGITS, embed_bits == 8, X, type, ldx, codes, scales, (half_t*)out, ldo, nullptr, nullptr, 0, B, L, d, 1, false,
                     reinterpret_cast<hipStream_t>(stream));
 }
 
@@ -216,7 +222,7 @@ static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
 
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K) {
   if (!dims_ok(B) || !dims_ok(L) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
-  if (K <= TOPK_MAX || mx_by_maxima(L, K)) return (size_t)B * (size_t)mx_maxima(L) * 4;
+  if (K <= TOPK_MAX || mx_by_maxima(L, K)) return (size_t)B * (size_t)mx_maxima(B, L, K) * 4;
   return mx_logit_rows_bytes(B, L, K);
 }
 
@@ -226,7 +232,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   if (rc || B == 0) return rc;
   if (K < 1 || K > SEL_MAX_K || L < K || numy < 1 || !values || !indices) return XFC_ERR_INVALID;
   const bool maxima = K <= TOPK_MAX || mx_by_maxima(L, K);
-  const int64_t least = B < 256 || maxima ? B : 256;
+  const int64_t least = B < 256 || maxima ? B : 256;  // rows
   if (!workspace || workspace_bytes < xfc_mx4_topk_workspace_bytes(least, L, K)) return XFC_ERR_WORKSPACE;
   if (!aligned16(workspace)) return XFC_ERR_ALIGN;
   const bool x8 = embed_bits == 8;
@@ -241,7 +247,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
       half_t* const logits = (half_t*)workspace;
       half_t* const hmax = select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? logits + round_up(rows * ldl, 8) : nullptr;
       rc = mx_product(MX_LOGITS_MAX, x8, reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type), type, ldx, codes, scales,
-                      logits, ldl, hmax, nullptr, ldb, rows, L, d, 1, st);
+                      logits, ldl, hmax, nullptr, ldb, rows, L, d, 1, false, st);
       if (rc) return rc;
       rc = select_rows(logits, ldl, (int)rows, (int)L, numy, K, hmax, ldb, values + r0 * K, indices + r0 * K, st);
       if (rc) return rc;
@@ -249,11 +255,14 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
     return XFC_OK;
   }
   float* const bmax = (float*)workspace;
-  const int64_t ldb = mx_maxima(L);
-  rc = mx_product(K > TOPK_MAX ? MX_HALF_MAXIMA : MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d, L >= (1 << 20) ? 4 : 1, st);
+  const int64_t ldb = mx_maxima(B, L, K);
+  const bool fine = mx_fine(B, K);
+  const int block = K > TOPK_MAX ? MX_SELECT_BLOCK : fine ? MX_UNIT / 2 : MX_UNIT;
+  rc = mx_product(K > TOPK_MAX ? MX_HALF_MAXIMA : MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d,
+                  !fine && L >= (1 << 20) ? 4 : 1, fine, st);
   if (rc) return rc;
   PickArgs k = {};
-  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, K > TOPK_MAX ? 32 : MX_UNIT); k.N = (int)L; k.K = (int)d; k.topk = K;
+  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, block); k.N = (int)L; k.K = (int)d; k.topk = K;
   k.begin = k.end = 1; k.numy = numy; k.out_v = values; k.out_i = indices;
   auto pick = [&](auto s) {
     using S = decltype(s);
@@ -263,7 +272,8 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
       hipLaunchKernelGGL(kernel, dim3((unsigned)B), dim3(MX_SELECT_THREADS), (unsigned)(S::lds(d) + sizeof(MxSelectLds)), st, k, s);
       return check_launch();
     }
-    hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 18 KB at most
+    if (fine) hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT / 2, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 11 KB at most
+    else hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);
     return check_launch();
   };
   if (x8) return pick(MxScores<true>{X, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales});

@@ -278,14 +278,16 @@ __device__ __forceinline__ const XFC_GLB uint8_t* scalar(const uint8_t* p) {
 }
 
 // MX_LOGITS: logits.  MX_LOGITS_MAX: the same for a selection, numbers only (a NaN becomes -inf), with the largest of every 32.
-// MX_MAXIMA: the largest sum of every unit.  MX_HALF_MAXIMA: the largest of every 32 as a logit, no number counts as -inf.
+// MX_MAXIMA: the largest sum of every unit, or of every half of one.  MX_HALF_MAXIMA: the largest of every 32 as a logit, no number counts
+// as -inf.
 enum MxOut { MX_LOGITS, MX_LOGITS_MAX, MX_MAXIMA, MX_HALF_MAXIMA };
 
 struct MxProductArgs {
   const void* X; int type; int64_t ldx;  // M rows of K
   const uint8_t* codes; const uint8_t* scales;
   half_t* out; int64_t ldo;              // logits
-  half_t* hmax; float* bmax; int64_t ldb; // beside logits; alone: a float or two halves for a unit
+  half_t* hmax; float* bmax; int64_t ldb; // beside logits; alone: one float for a unit, two, or two halves
+  bool fine;                              // MX_MAXIMA: of half units, which run = 1 alone has
   int M, N, K;
   int units, blocks, steps;
   int tiles_m, slots;                    // row tiles; workgroups of a row tile on an XCD
@@ -410,31 +412,40 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
       };
       // lane group g ends up with row tile 4 n + g
       auto over_lanes = [&](int n, auto of) { return fold16(fold32(of(4 * n), of(4 * n + 2)), fold32(of(4 * n + 1), of(4 * n + 3))); };
-      const int r4 = unit & (run - 1);
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        float m;
-        if constexpr (OUT == MX_MAXIMA) {
-          m = over_lanes(n, [&](int j) { return max_num(largest(j, 0), largest(j, 1)); });
-        } else {
-          typedef half_t half2v __attribute__((ext_vector_type(2)));
-          const float least = -__builtin_huge_valf();
-          const half2v two = {(half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 0); }), least),
-                              (half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 1); }), least)};
-          m = __builtin_bit_cast(float, two);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) best[n][r] = r4 == r ? m : best[n][r];
-      }
-      const int after = next(unit);
-      if (after != unit + 1 || run == 1 || after >= a.units) {
+      if (OUT == MX_MAXIMA && a.fine) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
+          const float m0 = over_lanes(n, [&](int j) { return largest(j, 0); }), m1 = over_lanes(n, [&](int j) { return largest(j, 1); });
           const int row = row0 + 64 * n + lane_now;
-          if (4 * n + q >= NT || row >= a.M) continue;
-          float* const to = a.bmax + (int64_t)row * a.ldb + (unit - r4);
-          if (run == 1) *to = best[n][0];
-          else *reinterpret_cast<float4v*>(to) = best[n];
+          if (4 * n + q < NT && row < a.M) *reinterpret_cast<float2v*>(a.bmax + (int64_t)row * a.ldb + 2 * (int64_t)unit) = float2v{m0, m1};
+        }
+      } else {
+        const int r4 = unit & (run - 1);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          float m;
+          if constexpr (OUT == MX_MAXIMA) {
+            m = over_lanes(n, [&](int j) { return max_num(largest(j, 0), largest(j, 1)); });
+          } else {
+            typedef half_t half2v __attribute__((ext_vector_type(2)));
+            const float least = -__builtin_huge_valf();
+            const half2v two = {(half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 0); }), least),
+                                (half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 1); }), least)};
+            m = __builtin_bit_cast(float, two);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) best[n][r] = r4 == r ? m : best[n][r];
+        }
+        const int after = next(unit);
+        if (after != unit + 1 || run == 1 || after >= a.units) {
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            const int row = row0 + 64 * n + lane_now;
+            if (4 * n + q >= NT || row >= a.M) continue;
+            float* const to = a.bmax + (int64_t)row * a.ldb + (unit - r4);
+            if (run == 1) *to = best[n][0];
+            else *reinterpret_cast<float4v*>(to) = best[n];
+          }
         }
       }
     } else {
@@ -503,12 +514,14 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
   }
 }
 
-// How topk_pick_kernel forms the scores of sixteen labels again: blocks are units, the sixteen are one of their four tiles.  The row, quantised once, stands in all sixteen columns; the MFMAs and their order are those of mx4_product_kernel.
+// The scores of sixteen labels of a row formed again, for topk_pick_kernel and below: any sixteen, each lane of the A side fetches its own.  The
+// row, quantised once, stands in all sixteen columns; a sum's MFMAs and their order are those of mx4_product_kernel.
 template <bool X8>
 struct MxScores {
   const void* X; int type; int64_t ldx;
   const uint8_t* codes; const uint8_t* scales;
 
+  static constexpr int MANY = 2;  // groups of labels whose fetches are on their way together
   static __device__ __forceinline__ unsigned char* room() {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
     return smem_raw;
@@ -519,7 +532,7 @@ struct MxScores {
 
   __device__ __forceinline__ void open(const PickArgs& a, int row) const {
     unsigned char* const at = room();
-    for (int w = threadIdx.x; w < mx_steps(a.K) * 16; w += 512) {
+    for (int w = threadIdx.x; w < mx_steps(a.K) * 16; w += blockDim.x) {
       const int part = w & 3, block = (w >> 2) & 3, step = w >> 4, k = w * 8;
       Float8 f = {};
       if (k < a.K) f = load8_of(X, type, (int64_t)row * ldx + k);
@@ -531,24 +544,36 @@ struct MxScores {
       if (part == 0) s[STEP_BYTES - 16 + block] = (unsigned char)byte;
     }
   }
-  static __device__ __forceinline__ int place(int part, int lane) { return mx_label(part, 4 * (lane >> 4)); }
-  __device__ __forceinline__ float4v score(const PickArgs& a, int, int first, int part, int lane) const {
+  // Labels first .. first + 15, first a multiple of 16: lane (., q) has four of them, first + 4 q on.
+  static __device__ __forceinline__ int place(int part, int lane) { return 16 * part + 4 * (lane >> 4); }
+  __device__ __forceinline__ void score(const PickArgs& a, const int (&first)[MANY], int lane, float4v (&z)[MANY]) const {
     const int blocks = mx_blocks(a.K), steps = mx_steps(a.K), i = lane & 15, q = lane >> 4;
-    const int64_t unit = first / MX_UNIT;
-    const uint8_t* const c = codes + unit * mx_code_bytes(a.K);
-    const uint8_t* const s = scales + unit * mx_scale_bytes(a.K);
     const unsigned char* const at = room();
-    float4v z = {0.f, 0.f, 0.f, 0.f};
-    constexpr int AT_ONCE = 6;  // steps whose fetches are on their way together
-    for (int s0 = 0; s0 < steps; s0 += AT_ONCE) {
-      int4v w[AT_ONCE];
-      uint32_t sa[AT_ONCE];
+    const uint8_t* c[MANY];
+    const uint8_t* s[MANY];
+    int tile[MANY], row[MANY];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int step = s0 + j < steps ? s0 + j : steps - 1, wide = blocks - 4 * step < 4 ? blocks - 4 * step : 4;
-        w[j] = *reinterpret_cast<const int4v*>(c + mx_code_at(part, i, 4 * step + (q < wide ? q : wide - 1), blocks));
-        sa[j] = *reinterpret_cast<const uint32_t*>(s + step * 256 + lane * 4) >> (8 * part);
-      }
+    for (int m = 0; m < MANY; ++m) {
+      const int64_t unit = first[m] / MX_UNIT;
+      const int within = first[m] % MX_UNIT + i;
+      tile[m] = mx_tile(within);
+      row[m] = mx_row(within);
+      c[m] = codes + unit * mx_code_bytes(a.K);
+      s[m] = scales + unit * mx_scale_bytes(a.K) + q * 64 + row[m] * 4 + tile[m];
+      z[m] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+    constexpr int AT_ONCE = 6;  // steps on their way together
+    for (int s0 = 0; s0 < steps; s0 += AT_ONCE) {
+      int4v w[MANY][AT_ONCE];
+      uint32_t sa[MANY][AT_ONCE];
+#pragma unroll
+      for (int m = 0; m < MANY; ++m)
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          const int step = s0 + j < steps ? s0 + j : steps - 1, wide = blocks - 4 * step < 4 ? blocks - 4 * step : 4;
+          w[m][j] = *reinterpret_cast<const int4v*>(c[m] + mx_code_at(tile[m], row[m], 4 * step + (q < wide ? q : wide - 1), blocks));
+          sa[m][j] = s[m][step * 256];
+        }
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
         if (s0 + j >= steps) break;
@@ -561,29 +586,34 @@ struct MxScores {
           const int4v lo = *reinterpret_cast<const int4v*>(x + q * 16);
           b = __builtin_shufflevector(lo, lo, 0, 1, 2, 3, -1, -1, -1, -1);
         }
-        z = mx_mfma<X8, 0, 0>(w[j], sa[j], b, x[STEP_BYTES - 16 + q], z);
+        const uint32_t sb = x[STEP_BYTES - 16 + q];
+#pragma unroll
+        for (int m = 0; m < MANY; ++m) z[m] = mx_mfma<X8, 0, 0>(w[m][j], sa[m][j], b, sb, z[m]);
       }
     }
-    return z;
   }
 };
 
 // ---------------------------------------------------------------------------------------------
-// 8 < K <= MX_SELECT_K without logits: the K best blocks of 32 by their maxima, their scores formed again
+// 8 < K <= MX_SELECT_K without logits: the K best blocks of 32 labels by their maxima, their scores formed again
 // ---------------------------------------------------------------------------------------------
 // Why that is exact: as in topk.hpp, with scores rounded to fp16; the K-th best maximum is no larger than the K-th best score, so
 // that of the K blocks' scores only those that reach it are put in order.
 //
-// One workgroup per row.  The maxima's keys are counted by their upper eleven bits, then those of the bin that the K-th is in by
-// the lower five; blocks above the K-th key are taken, and of those at it the first ones.  Sixteen waves then form the scores as MxScores
-// does, a tile of a block each.  Bound by fetching K x 32 labels a row.
-constexpr int MX_SELECT_K = 256, MX_SELECT_THREADS = 1024, MX_SELECT_BINS = 2048;
+// One workgroup per row.  The K-th largest of the threads' own largest maxima, to eleven bits, is no larger than the K-th maximum; the blocks that
+// reach it, a few more than K, are listed and ranked by comparing each with all.  Only if there is no room for them (rows of many
+// equal scores) are the maxima counted by their upper eleven bits and then, in the bin that the K-th is in, by the lower five, and of those
+// at the K-th key the first ones taken.  Sixteen waves then form the scores, a block at a time each.  Bound by fetching K x 32 labels
+// a row, after some 25 us for the blocks (512 rows x 40,960).  (Blocks of 16 would halve that, but their maxima cost the product more than they
+// save.)
+constexpr int MX_SELECT_K = 256, MX_SELECT_BLOCK = 32, MX_SELECT_THREADS = 1024, MX_SELECT_BINS = 2048;
 
-// (of PickArgs: bmax, two halves a float; n_blocks of 32 labels; N, K, topk, numy, out_v, out_i)
+// (of PickArgs: bmax, two halves a float; n_blocks; N, K, topk, numy, out_v, out_i)
 struct MxSelectLds {
-  unsigned long long cand[MX_SELECT_K * 32];
+  unsigned long long cand[MX_SELECT_K * MX_SELECT_BLOCK];
   int hist[MX_SELECT_BINS];
   int block[MX_SELECT_K];
+  unsigned long long list[MX_SELECT_THREADS];
   int wave_tot[MX_SELECT_THREADS / 64];
   int bin, above, n_block, n_cand;
 };
@@ -602,7 +632,7 @@ template <bool X8>
 __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs a, MxScores<X8> scores) {
   MxSelectLds& S = *reinterpret_cast<MxSelectLds*>(MxScores<X8>::room() + MxScores<X8>::lds(a.K));  // a multiple of 16
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int K = a.topk < a.n_blocks ? a.topk : a.n_blocks;  // blocks wanted
+  const int K = a.topk;  // there are more blocks
   const uint32_t* const maxima = reinterpret_cast<const uint32_t*>(a.bmax) + (int64_t)row * a.ldb;  // two blocks each
   const int quads = (a.n_blocks + 7) / 8;
   auto for_each = [&](auto&& f) {
@@ -640,77 +670,130 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
     }
     __syncthreads();
   };
+  // The same by counting all maxima; leaves the blocks and returns the K-th key.
+  auto by_counts = [&]() -> uint32_t {
+    for (int i = tid; i < MX_SELECT_BINS; i += MX_SELECT_THREADS) S.hist[i] = 0;
+    if (tid == 0) S.n_block = 0;
+    __syncthreads();
+    for_each([&](uint32_t key, int) { atomicAdd(&S.hist[key >> 5], 1); });
+    __syncthreads();
+    find_bin(MX_SELECT_BINS, 0);
+    const int top = S.bin, above = S.above;
+    __syncthreads();
+    if (tid < 64) S.hist[tid] = 0;
+    __syncthreads();
+    for_each([&](uint32_t key, int) { if ((int)(key >> 5) == top) atomicAdd(&S.hist[key & 31], 1); });
+    __syncthreads();
+    find_bin(64, above);
+    const uint32_t least = (uint32_t)top * 32 + (uint32_t)S.bin;
+    const int at_least = K - S.above;  // blocks at the K-th key that are taken, the first ones
+    // (the list's order is of no matter)
+    int taken = 0;
+    for (int w0 = 0; w0 < quads; w0 += MX_SELECT_THREADS) {
+      uint32_t here = 0, equal = 0;  // of this thread's eight blocks: above the key, at it
+      if (w0 + tid < quads) {
+        const uint4v v = *reinterpret_cast<const uint4v*>(maxima + 4 * (w0 + tid));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t key = half_key((v[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+          if (8 * (w0 + tid) + e < a.n_blocks) {
+            here |= (key > least ? 1u : 0u) << e;
+            equal |= (key == least ? 1u : 0u) << e;
+          }
+        }
+      }
+      // the equal ones' ranks, in the order of blocks
+      int mine = __builtin_popcount(equal), rank = mine;
+      const bool any = __syncthreads_or(mine != 0 && taken < at_least);
+      if (any) {
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int v = __shfl_up(rank, off, 64);
+          if (lane >= off) rank += v;
+        }
+        if (lane == 63) S.wave_tot[wave] = rank;
+        __syncthreads();
+        int before = taken, all = 0;
+        for (int w = 0; w < MX_SELECT_THREADS / 64; ++w) {
+          before += w < wave ? S.wave_tot[w] : 0;
+          all += S.wave_tot[w];
+        }
+        before += rank - mine;
+        for (uint32_t left = equal; left && before < at_least; left &= left - 1, ++before) here |= left & (0u - left);
+        taken += all;
+      }
+      for (; here; here &= here - 1) S.block[atomicAdd(&S.n_block, 1)] = 8 * (w0 + tid) + __builtin_ctz(here);
+      __syncthreads();
+    }
+    return least;
+  };
   for (int i = tid; i < MX_SELECT_BINS; i += MX_SELECT_THREADS) S.hist[i] = 0;
   if (tid == 0) S.n_block = S.n_cand = 0;
   scores.open(a, row);
+  uint32_t largest = 0;
+  for_each([&](uint32_t key, int) { largest = key > largest ? key : largest; });
   __syncthreads();
-  for_each([&](uint32_t key, int) { atomicAdd(&S.hist[key >> 5], 1); });
+  if (tid < quads) atomicAdd(&S.hist[largest >> 5], 1);
   __syncthreads();
   find_bin(MX_SELECT_BINS, 0);
-  const int top = S.bin, above = S.above;
+  const uint32_t bound = (uint32_t)S.bin * 32;
+  for_each([&](uint32_t key, int block) {
+    if (key < bound) return;
+    const int at = atomicAdd(&S.n_block, 1);
+    if (at < MX_SELECT_THREADS) S.list[at] = ((unsigned long long)key << 32) | (uint32_t)~block;
+  });
   __syncthreads();
-  if (tid < 64) S.hist[tid] = 0;
+  const int listed = S.n_block;
   __syncthreads();
-  for_each([&](uint32_t key, int) { if ((int)(key >> 5) == top) atomicAdd(&S.hist[key & 31], 1); });
-  __syncthreads();
-  find_bin(64, above);
-  const uint32_t least = (uint32_t)top * 32 + (uint32_t)S.bin;
-  const int at_least = K - S.above;  // blocks at the K-th key that are taken, the first ones
-  // (the list's order is of no matter)
-  int taken = 0;
-  for (int w0 = 0; w0 < quads; w0 += MX_SELECT_THREADS) {
-    uint32_t here = 0, equal = 0;  // of this thread's eight blocks: above the key, at it
-    if (w0 + tid < quads) {
-      const uint4v v = *reinterpret_cast<const uint4v*>(maxima + 4 * (w0 + tid));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = half_key((v[e >> 1] >> (16 * (e & 1))) & 0xffffu);
-        if (8 * (w0 + tid) + e < a.n_blocks) {
-          here |= (key > least ? 1u : 0u) << e;
-          equal |= (key == least ? 1u : 0u) << e;
-        }
-      }
+  uint32_t least;
+  if (listed <= MX_SELECT_THREADS) {
+    if (tid < listed) {
+      const unsigned long long mine = S.list[tid];
+      int rank = 0;
+      for (int o = 0; o < listed; ++o) rank += S.list[o] > mine;
+      if (rank < K) S.block[rank] = (int)~(uint32_t)mine;
+      if (rank == K - 1) S.bin = (int)(mine >> 32);
     }
-    // the equal ones' ranks, in the order of blocks
-    int mine = __builtin_popcount(equal), rank = mine;
-    const bool any = __syncthreads_or(mine != 0 && taken < at_least);
-    if (any) {
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int v = __shfl_up(rank, off, 64);
-        if (lane >= off) rank += v;
-      }
-      if (lane == 63) S.wave_tot[wave] = rank;
-      __syncthreads();
-      int before = taken, all = 0;
-      for (int w = 0; w < MX_SELECT_THREADS / 64; ++w) {
-        before += w < wave ? S.wave_tot[w] : 0;
-        all += S.wave_tot[w];
-      }
-      before += rank - mine;
-      for (uint32_t left = equal; left && before < at_least; left &= left - 1, ++before) here |= left & (0u - left);
-      taken += all;
-    }
-    for (; here; here &= here - 1) S.block[atomicAdd(&S.n_block, 1)] = 8 * (w0 + tid) + __builtin_ctz(here);
     __syncthreads();
+    least = (uint32_t)S.bin;
+  } else {
+    least = by_counts();
   }
-  const int n_block = S.n_block;  // K
-  for (int u = wave; u < 2 * n_block; u += MX_SELECT_THREADS / 64) {
-    const int first = S.block[u >> 1] * 32, part = 2 * ((first / 32) & 1) + (u & 1);
-    const float4v z = scores.score(a, row, first & ~(MX_UNIT - 1), part, lane);
-    if ((lane & 15) == 0) {
+  const int n_block = K;
+  for (int u = wave; u < n_block; u += MX_SELECT_THREADS / 64) {
+    const int block = __builtin_amdgcn_readfirstlane(S.block[u]) * MX_SELECT_BLOCK;
+    const int first[2] = {block, block + 16};
+    float4v z[2];
+    scores.score(a, first, lane, z);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if ((lane & 15) != 0) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int label = (first & ~(MX_UNIT - 1)) + mx_label(part, 4 * (lane >> 4) + r);
-        const half_t h = z[r] == z[r] ? (half_t)z[r] : (half_t)-__builtin_huge_valf();
+        const int label = first[m] + 4 * (lane >> 4) + r;
+        const half_t h = z[m][r] == z[m][r] ? (half_t)z[m][r] : (half_t)-__builtin_huge_valf();
         const uint32_t key = half_key(__builtin_bit_cast(uint16_t, h));
-        if (label < a.N && (key >= least || n_block < a.topk)) S.cand[atomicAdd(&S.n_cand, 1)] = ((unsigned long long)key << 32) | (uint32_t)~label;
+        if (label < a.N && key >= least) S.cand[atomicAdd(&S.n_cand, 1)] = ((unsigned long long)key << 32) | (uint32_t)~label;
       }
     }
   }
   __syncthreads();
-  // in order: bitonic over the next power of two
+  auto write = [&](int at, unsigned long long c) {
+    const int64_t label = (int64_t)(uint32_t)~(uint32_t)c;
+    a.out_v[(int64_t)row * K + at] = half_unkey((uint32_t)(c >> 32));
+    a.out_i[(int64_t)row * K + at] = label < a.numy ? label : a.numy - 1;
+  };
   const int n = S.n_cand;
+  if (n <= MX_SELECT_THREADS) {
+    if (tid < n) {
+      const unsigned long long mine = S.cand[tid];
+      int rank = 0;
+      for (int o = 0; o < n; ++o) rank += S.cand[o] > mine;
+      if (rank < K) write(rank, mine);
+    }
+    return;
+  }
+  // bitonic over the next power of two
   int size = 64;
   while (size < n) size <<= 1;
   for (int i = n + tid; i < size; i += MX_SELECT_THREADS) S.cand[i] = 0;
@@ -726,12 +809,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
       }
       __syncthreads();
     }
-  for (int i = tid; i < a.topk; i += MX_SELECT_THREADS) {
-    const unsigned long long c = S.cand[i];
-    const int64_t label = (int64_t)(uint32_t)~(uint32_t)c;
-    a.out_v[(int64_t)row * a.topk + i] = half_unkey((uint32_t)(c >> 32));
-    a.out_i[(int64_t)row * a.topk + i] = label < a.numy ? label : a.numy - 1;
-  }
+  for (int i = tid; i < K; i += MX_SELECT_THREADS) write(i, S.cand[i]);
 }
 
 }  // namespace xfc

@@ -362,7 +362,9 @@ __device__ __forceinline__ unsigned long long wave_top(unsigned long long key, i
 
 // How topk_pick_kernel forms the scores of 16 labels of a block again: half weights.  open() runs once, before the first score and
 // a barrier; score() leaves four labels' scores in every lane, of which lanes 0, 16, 32 and 48 are kept, at place() in the block.
+// (Where MANY is more than one, of as many groups of 16 labels at a time.)
 struct HalfScores {
+  static constexpr int MANY = 1;
   static constexpr int STEPS = 8;  // pieces of the weights on their way
   __device__ __forceinline__ void open(const PickArgs&, int) const {}
   static __device__ __forceinline__ int place(int part, int lane) { return part * 16 + 4 * (lane >> 4); }
@@ -486,10 +488,30 @@ __global__ void __launch_bounds__(512) topk_pick_kernel(PickArgs a, Scores score
     for (int r = 0; r < K; ++r) n_sel += chosen[r] != 0;
     n_sel = __builtin_amdgcn_readfirstlane(n_sel);
     // their scores, 16 labels at a time; the MFMAs and their order are those of the kernels above
-    for (int u = wave; u < n_sel * (BLOCK / 16); u += NW) {
-      const int part = u % (BLOCK / 16);
-      const float4v z = scores.score(a, row, (int)~(uint32_t)chosen[u / (BLOCK / 16)] * BLOCK, part, lane);
-      if ((lane & 15) == 0) *reinterpret_cast<float4v*>(&score[u / (BLOCK / 16) * BLOCK + Scores::place(part, lane)]) = z;
+    constexpr int MANY = Scores::MANY;
+    if constexpr (MANY == 1) {
+      for (int u = wave; u < n_sel * (BLOCK / 16); u += NW) {
+        const int part = u % (BLOCK / 16);
+        const float4v z = scores.score(a, row, (int)~(uint32_t)chosen[u / (BLOCK / 16)] * BLOCK, part, lane);
+        if ((lane & 15) == 0) *reinterpret_cast<float4v*>(&score[u / (BLOCK / 16) * BLOCK + Scores::place(part, lane)]) = z;
+      }
+    } else {
+      const int all = n_sel * (BLOCK / 16);
+      for (int u = wave; u < all; u += MANY * NW) {
+        int first[MANY];
+        float4v z[MANY];
+#pragma unroll
+        for (int m = 0; m < MANY; ++m) {
+          const int v = u + m * NW < all ? u + m * NW : u;
+          first[m] = __builtin_amdgcn_readfirstlane((int)~(uint32_t)chosen[v / (BLOCK / 16)]) * BLOCK + v % (BLOCK / 16) * 16;
+        }
+        scores.score(a, first, lane, z);
+#pragma unroll
+        for (int m = 0; m < MANY; ++m) {
+          const int v = u + m * NW;
+          if ((lane & 15) == 0 && v < all) *reinterpret_cast<float4v*>(&score[v / (BLOCK / 16) * BLOCK + Scores::place(v % (BLOCK / 16), lane)]) = z[m];
+        }
+      }
     }
     __syncthreads();
     // the K best of the blocks' labels and of what was there before
