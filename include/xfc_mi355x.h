@@ -316,7 +316,7 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
  * Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, K); where logits are written and there are more than 256 rows, what 256
  * rows take is enough, the rows then go in turns.
  */
-size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K);
+size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t d, int64_t K);
 int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,
                  int64_t numy, int K, int embed_bits, float* values, int64_t* indices, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -51,7 +51,7 @@ _SIGNATURES = {
     "xfc_mx4_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
     "xfc_mx4_dequantize": (_int, [_vp, _vp, _i64, _i64, _vp, _int, _i64, _vp]),
     "xfc_mx4_logits": (_int, [_vp, _int, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
-    "xfc_mx4_topk_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "xfc_mx4_topk_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "xfc_mx4_topk": (_int, [_vp, _int, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _sz, _vp]),
     "xfc_preference_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "xfc_preference": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _f32, _f32,

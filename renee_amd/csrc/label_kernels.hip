@@ -212,17 +212,22 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
                     reinterpret_cast<hipStream_t>(stream));
 }
 
-// K > 8: by logits, or by maxima of 32 labels and the K best blocks' scores formed again.
-static bool mx_by_maxima(int64_t L, int64_t K) { return K <= MX_SELECT_K && L >= 4096 * K; }
+// K > 8: by logits, or by maxima of 32 labels and the K best blocks' scores formed again.  Writing logits takes 2 L bytes a row, fetching the blocks 17 d K;
+// a row's blocks are one workgroup's, which few rows wait for.  (us by maxima / by logits.  512 rows x 768 dims: 131,072 labels, K = 10 67 / 74,
+// 50 106 / 80; 320,001, K = 50 145 / 179, 100 189 / 180; 1,310,720, K = 200 481 / 650.  x 64: 131,072, K = 100 54 / 58, 200 78 / 66.  32 rows x 768:
+// 131,072, K = 10 28 / 30; 1,310,720, K = 50 154 / 169, 100 174 / 171.  1 row x 1,310,720 x 768, K = 10 130 / 109.)
+static bool mx_by_maxima(int64_t B, int64_t L, int64_t d, int64_t K) {
+  return K > TOPK_MAX && K <= MX_SELECT_K && B >= 32 && L >= (B < 128 ? 2 : 1) * K * (1000 + 5 * d);
+}
 // By logits: those of this many rows, and the maxima of their blocks
 static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
-  const size_t logits = (size_t)rows * (size_t)round_up(L, 8) * 2;
+  const size_t logits = (size_t)rows * (size_t)round_up(L, MX_UNIT) * 2;
   return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_half_maxima(L) * 2 : 0);
 }
 
-size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t K) {
-  if (!dims_ok(B) || !dims_ok(L) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
-  if (K <= TOPK_MAX || mx_by_maxima(L, K)) return (size_t)B * (size_t)mx_maxima(B, L, K) * 4;
+size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t d, int64_t K) {
+  if (!dims_ok(B) || !dims_ok(L) || !dims_ok(d) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
+  if (K <= TOPK_MAX || mx_by_maxima(B, L, d, K)) return (size_t)B * (size_t)mx_maxima(B, L, K) * 4;
   return mx_logit_rows_bytes(B, L, K);
 }
 
@@ -231,21 +236,21 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   int rc = check_product(X, type, ldx, codes, scales, B, L, d, embed_bits);
   if (rc || B == 0) return rc;
   if (K < 1 || K > SEL_MAX_K || L < K || numy < 1 || !values || !indices) return XFC_ERR_INVALID;
-  const bool maxima = K <= TOPK_MAX || mx_by_maxima(L, K);
-  const int64_t least = B < 256 || maxima ? B : 256;  // rows
-  if (!workspace || workspace_bytes < xfc_mx4_topk_workspace_bytes(least, L, K)) return XFC_ERR_WORKSPACE;
+  const bool maxima = K <= TOPK_MAX || mx_by_maxima(B, L, d, K);
+  const size_t need = xfc_mx4_topk_workspace_bytes(B, L, d, K), turn = mx_logit_rows_bytes(256, L, K);  // all rows, 256 rows' logits
+  if (!workspace || workspace_bytes < (maxima || B <= 256 ? need : turn)) return XFC_ERR_WORKSPACE;
   if (!aligned16(workspace)) return XFC_ERR_ALIGN;
   const bool x8 = embed_bits == 8;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (!maxima) {
     const int64_t ldb = mx_half_maxima(L);
     int64_t block = B;
-    if (workspace_bytes < xfc_mx4_topk_workspace_bytes(B, L, K)) block = (int64_t)(workspace_bytes / xfc_mx4_topk_workspace_bytes(256, L, K)) * 256;
-    const int64_t ldl = round_up(L, 8);
+    if (workspace_bytes < need) block = (int64_t)(workspace_bytes / turn) * 256;
+    const int64_t ldl = round_up(L, MX_UNIT);
     for (int64_t r0 = 0; r0 < B; r0 += block) {
       const int64_t rows = B - r0 < block ? B - r0 : block;
       half_t* const logits = (half_t*)workspace;
-      half_t* const hmax = select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? logits + round_up(rows * ldl, 8) : nullptr;
+      half_t* const hmax = select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? logits + rows * ldl : nullptr;
       rc = mx_product(MX_LOGITS_MAX, x8, reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type), type, ldx, codes, scales,
                       logits, ldl, hmax, nullptr, ldb, rows, L, d, 1, false, st);
       if (rc) return rc;

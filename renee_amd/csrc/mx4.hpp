@@ -296,6 +296,29 @@ struct MxProductArgs {
 
 constexpr int MX_WAVES = 8, MX_SLOTS = 3;
 
+// The first n of eight halves, to a place that begins on 16 bytes.
+__device__ __forceinline__ void store_first(half_t* to, const half8& h, int n) {
+  const uint4v v = __builtin_bit_cast(uint4v, h);
+  if (n >= 8) {
+    *reinterpret_cast<uint4v*>(to) = v;
+  } else if (n > 0) {
+    typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+    uint2v left = {v[0], v[1]};
+    if (n & 4) {
+      *reinterpret_cast<uint2v*>(to) = left;
+      left = uint2v{v[2], v[3]};
+      to += 4;
+    }
+    uint32_t last = left[0];
+    if (n & 2) {
+      *reinterpret_cast<uint32_t*>(to) = last;
+      last = left[1];
+      to += 2;
+    }
+    if (n & 1) *reinterpret_cast<uint16_t*>(to) = (uint16_t)last;
+  }
+}
+
 // A workgroup keeps its rows' fragments in the LDS and its waves, which never meet again, stream units of 64 labels past them, straight
 // into the A side's registers: MX_SLOTS - 1 steps on their way, across units.
 template <int NT, bool X8, int OUT>
@@ -462,7 +485,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
           }
         }
         const int row = row0 + 16 * j + i;
-        if (!edge) {
+        if (OUT == MX_LOGITS_MAX || !edge) {  // (a selection's rows have room for whole units)
           // Neighbouring lanes swap halves: a store is eight rows of 128 bytes, whole lines, where it was sixteen of 64.  (512 x 1,310,720 x
           // 768: 588 -> 529 us.  Past the caches they take as long.)
           const bool odd = i & 1;
@@ -480,15 +503,18 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
           if (first + 1 < a.M) *reinterpret_cast<uint4v*>(to + a.ldo) = odd_row;
         } else if (row < a.M) {
 #pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int col = label0 + 32 * p + 8 * q + e;
-              if (col < a.N) a.out[(int64_t)row * a.ldo + col] = h[p][e];
-              else h[p][e] = (half_t)-__builtin_huge_valf();
-            }
+          for (int p = 0; p < 2; ++p) {
+            const int col = label0 + 32 * p + 8 * q;
+            store_first(a.out + (int64_t)row * a.ldo + col, h[p], a.N - col);
+          }
         }
         if constexpr (OUT == MX_LOGITS_MAX) {
+          if (edge) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) h[p][e] = label0 + 32 * p + 8 * q + e < a.N ? h[p][e] : (half_t)-__builtin_huge_valf();
+          }
           const uint32_t v = pk_fold32(pk_max(h[0]), pk_max(h[1]));
           const half_t m = pk_larger(pk_fold16(v, v));
           if (a.hmax && row < a.M && (q & 1) == 0) a.hmax[(int64_t)row * a.ldb + 2 * (int64_t)unit + (q >> 1)] = m;
@@ -497,20 +523,23 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     }
   };
 
-  while (unit < a.units) {
-#pragma unroll
-    for (int s = 0; s < MX_SLOTS; ++s) {
-      if (unit < a.units) {
-        if (step == 0) multiply(slot[s], std::true_type{});
-        else multiply(slot[s], std::false_type{});
-        if (++step == a.steps) {
-          epilogue();
-          step = 0;
-          unit = next(unit);
-        }
+  auto turn = [&](Slot& w) {
+    if (unit < a.units) {
+      if (step == 0) multiply(w, std::true_type{});
+      else multiply(w, std::false_type{});
+      if (++step == a.steps) {
+        epilogue();
+        step = 0;
+        unit = next(unit);
       }
-      fetch(slot[s]);  // (whatever way was taken: else the compiler could not tell how many are on their way, and would wait for all)
     }
+    fetch(w);  // (whatever way was taken: else the compiler could not tell how many are on their way, and would wait for all)
+  };
+  static_assert(MX_SLOTS == 3, "turns");
+  while (unit < a.units) {  // (written out: a loop of this size would stay one, with the slots in scratch memory)
+    turn(slot[0]);
+    turn(slot[1]);
+    turn(slot[2]);
   }
 }
 

@@ -155,9 +155,7 @@ class MX4Labels:
         if bsz == 0:
             return values, indices
         L = lib()
-        need = L.xfc_mx4_topk_workspace_bytes(bsz, self.numy, K)
-        if need > 1 << 32 and K > 8:  # the logits of some rows at a time
-            need = max(min(need, 1 << 32), L.xfc_mx4_topk_workspace_bytes(min(bsz, 256), self.numy, K))
+        need = L.xfc_mx4_topk_workspace_bytes(bsz, self.numy, self.dims, K)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         with _On(self.device) as stream:
             rc = L.xfc_mx4_topk(x.data_ptr(), TYPES[x.dtype], x.stride(0), self.codes.data_ptr(), self.scales.data_ptr(), bsz, self.numy,

@@ -131,9 +131,9 @@ def test_topk_with_4_bits(dev, B, L, d, K):
     assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
 
 
-# (above 8 by maxima alone from 4096 K labels on)
-@pytest.mark.parametrize("B,L,d,K", [(2, 70001, 64, 5), (40, 66000, 128, 100), (5, 140003, 64, 8), (3, 70001, 64, 3000), (1, 36864, 8, 9), (130, 40961, 72, 10),
-                                     (33, 70001, 200, 16), (3, 414001, 64, 100), (2, 1050003, 32, 256)])
+# (above 8 by maxima alone from 32 rows and 1000 K or more labels on, here 36, 130 and 33 rows)
+@pytest.mark.parametrize("B,L,d,K", [(2, 70001, 64, 5), (40, 66000, 128, 100), (5, 140003, 64, 8), (3, 70001, 64, 3000), (36, 18729, 8, 9), (130, 40961, 72, 10),
+                                     (33, 70001, 200, 16), (3, 414001, 64, 100), (34, 600003, 8, 256), (130, 270011, 8, 256)])
 def test_topk_of_many_labels(dev, B, L, d, K):
     x, w, z = _problem(B, L, d, 4, torch.float16, L + K)
     v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=4)
@@ -169,14 +169,15 @@ def test_topk_ties_go_to_the_lower_label_and_constant_rows(dev):
 
 
 @pytest.mark.parametrize("K", [9, 12])
-@pytest.mark.parametrize("L", [1000, 50003])
+@pytest.mark.parametrize("L", [1000, 32003])
 def test_topk_above_8_counts_nan_as_the_least(dev, L, K):
     """Rows of equal scores, of fewer numbers than K, of none, and of infinities."""
     w = torch.zeros(L, 64, dtype=torch.float16)
     w[:, 0] = torch.randint(-2, 3, (L,), generator=torch.Generator().manual_seed(L)).half()
     w[5::3] = float("nan")
     w[:, 40] = torch.where(torch.arange(L) % 1009 == 7, 6.0e4, 0.0).half()
-    x = torch.zeros(5, 64, dtype=torch.float32)
+    x = torch.zeros(40, 64, dtype=torch.float32)  # by maxima with 32,003 labels
+    x[5:, 2] = 1.0
     x[0, 0], x[1, 1], x[2, 0], x[3, 40], x[4, 40] = 1.0, 1.0, float("nan"), 1e30, -1e30
     some = w.clone()
     some[4:] = float("nan")
@@ -204,7 +205,7 @@ def test_topk_rows_in_turns(dev):
     x, w, z = _problem(600, 3000, 64, 4, torch.float16, 33)
     labels, xd = MX4Labels.from_weight(w.to(dev)), x.to(dev)
     ev, ei = labels.topk(xd, 20, embed_bits=4)
-    need = lib().xfc_mx4_topk_workspace_bytes(256, 3000, 20)
+    need = lib().xfc_mx4_topk_workspace_bytes(256, 3000, 64, 20)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     v, i = torch.empty_like(ev), torch.empty_like(ei)
     check(lib().xfc_mx4_topk(xd.data_ptr(), 0, 64, labels.codes.data_ptr(), labels.scales.data_ptr(), 600, 3000, 64, 3000, 20, 4, v.data_ptr(),
