@@ -294,7 +294,7 @@ struct MxProductArgs {
   int run;                               // units in a row that a wave takes, 1 or 4
 };
 
-constexpr int MX_WAVES = 8, MX_SLOTS = 3;
+constexpr int MX_WAVES = 8, MX_SLOTS = 2;
 
 // The first n of eight halves, to a place that begins on 16 bytes.
 __device__ __forceinline__ void store_first(half_t* to, const half8& h, int n) {
@@ -320,7 +320,8 @@ __device__ __forceinline__ void store_first(half_t* to, const half8& h, int n) {
 }
 
 // A workgroup keeps its rows' fragments in the LDS and its waves, which never meet again, stream units of 64 labels past them, straight
-// into the A side's registers: MX_SLOTS - 1 steps on their way, across units.
+// into the A side's registers: two steps on their way, across units.  (Three or six took as long where there is much to do, and longer where
+// there is little, by the size of the code: 16 rows x 131,072 labels 12.8, 13.5, 17.7 us.)
 template <int NT, bool X8, int OUT>
 __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_kernel(MxProductArgs a) {
   using Rows = MxRows<X8>;
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
   int f_unit = unit < a.units ? unit : a.units - 1, f_step = 0;
   struct Slot { int4v w[MX_TILES]; uint32_t s; };
   Slot slot[MX_SLOTS];
-  auto fetch = [&](Slot& to) {
+  auto fetch = [&](Slot& to) __attribute__((always_inline)) {
     const uint8_t* const c = a.codes + (int64_t)f_unit * unit_codes + f_step * 4096;
     const uint8_t* const s = a.scales + (int64_t)f_unit * unit_scales + f_step * 256;
     const bool rest = f_step == whole;
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
   };
   [&]<int... J>(std::integer_sequence<int, J...>) { (read_rows(0, std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, AHEAD>{});
   read_scales(0, sb[0]);
-  auto multiply = [&](const Slot& w, auto first) {
+  auto multiply = [&](const Slot& w, auto first) __attribute__((always_inline)) {
     const int after = step + 1 == a.steps ? 0 : step + 1;
     read_scales(after, sb[1]);
     auto row_tile = [&](auto jt) {
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     for (int n = 0; n < NS; ++n) sb[0][n] = sb[1][n];
   };
 
-  auto epilogue = [&]() {
+  auto epilogue = [&]() __attribute__((always_inline)) {
     // (Made anew each time: kept over the loop, the rows' addresses would take the registers of the fragments under way.)
     int lane_now = lane;
     asm volatile("" : "+v"(lane_now));
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     }
   };
 
-  auto turn = [&](Slot& w) {
+  auto turn = [&](Slot& w) __attribute__((always_inline)) {
     if (unit < a.units) {
       if (step == 0) multiply(w, std::true_type{});
       else multiply(w, std::false_type{});
@@ -535,11 +536,10 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     }
     fetch(w);  // (whatever way was taken: else the compiler could not tell how many are on their way, and would wait for all)
   };
-  static_assert(MX_SLOTS == 3, "turns");
+  static_assert(MX_SLOTS == 2, "turns");
   while (unit < a.units) {  // (written out: a loop of this size would stay one, with the slots in scratch memory)
     turn(slot[0]);
     turn(slot[1]);
-    turn(slot[2]);
   }
 }
 
