@@ -143,6 +143,45 @@ __device__ __forceinline__ uint64_t to_fp8(Float8 f, float by) {
   hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, f.v[6], f.v[7], by, true);
   return (uint64_t)__builtin_bit_cast(uint32_t, lo) | ((uint64_t)__builtin_bit_cast(uint32_t, hi) << 32);
 }
+// The same of eight halves, without making floats of them: half the instructions.  Their blocks' scales are normal floats.
+template <int EMAX>
+__device__ __forceinline__ uint32_t block_scale(const half8& h, float& by) {
+  typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+  const uint4v q = __builtin_bit_cast(uint4v, h) & 0x7fff7fffu;
+  auto larger = [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, a), __builtin_bit_cast(ushort2v, b)));
+  };
+  const uint32_t two = larger(larger(q[0], q[1]), larger(q[2], q[3]));
+  const uint32_t m = quad_max((two >> 16) > (two & 0xffffu) ? two >> 16 : two & 0xffffu);
+  const uint32_t exponent = __float_as_uint((float)__builtin_bit_cast(half_t, (uint16_t)m)) >> 23;
+  const uint32_t byte = exponent - EMAX;  // (m = 0: not used)
+  by = m == 0 ? 1.f : __uint_as_float((exponent == 255 ? 127u : byte) << 23);
+  return exponent == 255 ? MX_NAN : m == 0 ? 0 : byte;
+}
+__device__ __forceinline__ uint32_t to_fp4(const half8& h, float by) {
+  typedef half_t half2v __attribute__((ext_vector_type(2)));
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2v{h[0], h[1]}, by, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2v{h[2], h[3]}, by, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2v{h[4], h[5]}, by, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, half2v{h[6], h[7]}, by, 3);
+}
+// (448 times the scale is a half, or rounds to one that no number of the block exceeds.)
+__device__ __forceinline__ uint64_t to_fp8(const half8& h, float by) {
+  typedef short short2v __attribute__((ext_vector_type(2)));
+  typedef half_t half2v __attribute__((ext_vector_type(2)));
+  const half_t most = (half_t)(448.f * by);
+  half8 c;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = most;
+  c = __builtin_elementwise_max(__builtin_elementwise_min(h, c), -c);
+  short2v lo = {0, 0}, hi = {0, 0};
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(lo, half2v{c[0], c[1]}, by, false);
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(lo, half2v{c[2], c[3]}, by, true);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(hi, half2v{c[4], c[5]}, by, false);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(hi, half2v{c[6], c[7]}, by, true);
+  return (uint64_t)__builtin_bit_cast(uint32_t, lo) | ((uint64_t)__builtin_bit_cast(uint32_t, hi) << 32);
+}
 // 2^(byte - 127), NaN for 255
 __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __uint_as_float(byte == MX_NAN ? 0x7fc00000u : byte == 0 ? 0x00400000u : byte << 23);
@@ -235,8 +274,9 @@ struct MxRows {
     if constexpr (X8) return (block >> 1) * 1024 + ((2 * (block & 1) + (part >> 1)) * 16 + i) * 16 + (part & 1) * 8;
     else return (block * 16 + i) * 16 + part * 4;
   }
-  // Quantises them (four neighbouring lanes hold a block) and returns the scale byte.
-  static __device__ __forceinline__ uint32_t put(unsigned char* frag, Float8 f, int i, int block, int part) {
+  // Quantises them (four neighbouring lanes hold a block; V: Float8 or half8) and returns the scale byte.
+  template <class V>
+  static __device__ __forceinline__ uint32_t put(unsigned char* frag, V f, int i, int block, int part) {
     float by;
     const uint32_t byte = block_scale<EMAX>(f, by);
     if constexpr (X8) *reinterpret_cast<uint64_t*>(frag + at(i, block, part)) = to_fp8(f, by);
@@ -361,16 +401,33 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
 #pragma unroll
   for (int s = 0; s < MX_SLOTS; ++s) fetch(slot[s]);
 
-  // The rows' blocks, four lanes each, 16 lanes a step of a row; behind the last row, dim or block there are zeros.
-  for (int w = tid; w < a.steps * NT * 256; w += 64 * MX_WAVES) {
-    const int part = w & 3, block = (w >> 2) & 3, step = (w >> 4) % a.steps, r = (w >> 4) / a.steps;
-    const int k = step * MX_STEP + block * MX_BLOCK + part * 8;
-    Float8 f = {};
-    if (row0 + r < a.M && k < a.K) f = load8_of(a.X, a.type, (int64_t)(row0 + r) * a.ldx + k);
-    const int j = r >> 4;
-    const uint32_t byte = Rows::put(frags + (step * NT + j) * Rows::FRAG, f, r & 15, block, part);
-    if (part == 0) row_scales[((step * NS + (j >> 2)) * 64 + block * 16 + (r & 15)) * 4 + (j & 3)] = (unsigned char)byte;
-  }
+  // The rows' blocks, four lanes each, 16 lanes a step of a row, 32 rows at a time, FILL steps on their way; behind the last row, dim or
+  // block there are zeros.
+  constexpr int FILL = 3;
+  auto fill = [&](auto load) __attribute__((always_inline)) {
+    const int part = tid & 3, block = (tid >> 2) & 3, k = block * MX_BLOCK + part * 8;
+    for (int r = tid >> 4; r < 16 * NT; r += 4 * MX_WAVES) {
+      const int j = r >> 4;
+      for (int s0 = 0; s0 < a.steps; s0 += FILL) {
+        decltype(load((int64_t)0)) v[FILL];
+#pragma unroll
+        for (int n = 0; n < FILL; ++n) {
+          v[n] = {};
+          if (row0 + r < a.M && (s0 + n) * MX_STEP + k < a.K) v[n] = load((int64_t)(row0 + r) * a.ldx + (s0 + n) * MX_STEP + k);
+        }
+#pragma unroll
+        for (int n = 0; n < FILL; ++n) {
+          const int step = s0 + n;
+          if (step >= a.steps) break;
+          const uint32_t byte = Rows::put(frags + (step * NT + j) * Rows::FRAG, v[n], r & 15, block, part);
+          if (part == 0) row_scales[((step * NS + (j >> 2)) * 64 + block * 16 + (r & 15)) * 4 + (j & 3)] = (unsigned char)byte;
+        }
+      }
+    }
+  };
+  if (a.type == XFC_F16) fill([&](int64_t at) { return *reinterpret_cast<const half8*>(reinterpret_cast<const half_t*>(a.X) + at); });
+  else if (a.type == XFC_BF16) fill([&](int64_t at) { return load8<XFC_BF16>(reinterpret_cast<const uint16_t*>(a.X) + at); });
+  else fill([&](int64_t at) { return load8<XFC_F32>(reinterpret_cast<const float*>(a.X) + at); });
   __syncthreads();
 
   float4v acc[MX_TILES][NT];
