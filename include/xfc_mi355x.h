@@ -335,7 +335,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
  * X: fp16, bf16 or fp32.  W: fp16 rows, or with scales non-NULL MX4 codes (ldw is not used).  reference, weight, margin, dX, G may be NULL
  * (0, 1, not wanted).  A pair with a label outside [0, L) or weight 0 is not there, whatever else it holds: its margin is 0, and so is
  * that of pairs which no row has.  Row pointers that do not ascend give an unspecified result for the rows of these pairs.  Results do not depend on
- * anything but the arguments: no atomics.  d <= 4096, a multiple of 8.
+ * anything but the arguments: no atomics.  d <= 4096, a multiple of 8; P <= 2^30.
  */
 size_t xfc_preference_workspace_bytes(int64_t B, int64_t P, int64_t d);
 int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t ldw, const void* scales, int64_t L, int64_t d,

@@ -1,6 +1,7 @@
 // Narrow label matrices and label preferences: the C entry points of mx4.hpp and preference.hpp.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <math.h>
 #include <stdio.h>
 
 #include "../../include/xfc_mi355x.h"
@@ -304,11 +305,11 @@ int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t 
                    void* dX, int dx_type, int64_t lddx, void* G, int64_t ldg, void* workspace, size_t workspace_bytes, void* stream) {
   if (!dims_ok(B) || !dims_ok(L) || !dims_ok(d) || !dims_ok(P) || !type_ok(type) || (dX && !type_ok(dx_type))) return XFC_ERR_INVALID;
   if (!loss || (B > 0 && (!X || !W || !rowptr)) || (P > 0 && (!chosen || !rejected)) || d <= 0 || L <= 0 || B > 0x7fffff) return XFC_ERR_INVALID;
-  if (!(beta == beta) || !(smoothing >= 0.f && smoothing <= 1.f)) return XFC_ERR_INVALID;
+  if (!(fabsf(beta) <= 3.4e38f) || !(smoothing >= 0.f && smoothing <= 1.f)) return XFC_ERR_INVALID;
   if (B > 0 && (d % 8 || !rows_ok(X, type, ldx) || !aligned16(W) || (scales ? !aligned16(scales) : ldw % 8 != 0) ||
                 (dX && !rows_ok(dX, dx_type, lddx)))) return XFC_ERR_ALIGN;
   if (B > 0 && (ldx < d || (!scales && ldw < d) || (dX && lddx < d) || (G && ldg < L))) return XFC_ERR_SHAPE;
-  if (d > 4096) return XFC_ERR_LIMIT;
+  if (d > 4096 || P > (1 << 30)) return XFC_ERR_LIMIT;
   if (!workspace || workspace_bytes < xfc_preference_workspace_bytes(B, P, d)) return XFC_ERR_WORKSPACE;
   if (!aligned16(workspace)) return XFC_ERR_ALIGN;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -332,7 +333,7 @@ int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t 
     if (rc) return rc;
   }
   const bool rows = B > 0 && (G || dX);
-  return launch_k<preference_finish_kernel>(dim3((unsigned)(rows ? B + 1 : 1)), dim3(PREF_FINISH), 0, st, a);
+  return launch_k<preference_finish_kernel>(dim3((unsigned)(rows ? B + 1 : 1)), dim3(rows && !G ? 256 : PREF_FINISH), 0, st, a);
 }
 
 }  // extern "C"

@@ -17,7 +17,7 @@ namespace xfc {
 
 constexpr int PREF_WAVES = 4;
 constexpr int pref_pairs(int pieces) { return pieces <= 2 ? 4 : 8 / pieces; }  // as many as the registers hold
-constexpr int PREF_FINISH = 1024;
+constexpr int PREF_FINISH = 1024;  // threads of a row with G
 constexpr int PREF_TILE = 512;  // pairs of a row whose entries of G are joined at a time
 
 struct PrefArgs {
@@ -200,16 +200,16 @@ __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs
   __shared__ __attribute__((aligned(16))) int32_t label[2 * PREF_TILE];
   __shared__ __attribute__((aligned(16))) float slope[2 * PREF_TILE];
   __shared__ double sums[PREF_FINISH / 64];
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
   if (row == (int)gridDim.x - 1) {
     double t = 0.0;
-    for (int i = tid; i < a.chunks; i += PREF_FINISH) t += a.part_loss[i];
+    for (int i = tid; i < a.chunks; i += threads) t += a.part_loss[i];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
     if ((tid & 63) == 0) sums[tid >> 6] = t;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 1; w < PREF_FINISH / 64; ++w) t += sums[w];
+      for (int w = 1; w < threads / 64; ++w) t += sums[w];
       *a.loss = (float)t;
     }
     return;
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs
   if (a.dX) {
     const int first = begin / a.chunk, last = end > begin ? (end - 1) / a.chunk : first;
     if (begin == end || first < last) {
-      for (int k = 8 * tid; k < a.d; k += 8 * PREF_FINISH) {
+      for (int k = 8 * tid; k < a.d; k += 8 * threads) {
         Float8 t = {};
         if (begin < end) {
           for (int c = first; c <= last; ++c) {
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs
   for (int p0 = begin; p0 < end; p0 += PREF_TILE) {
     const int n = end - p0 < PREF_TILE ? end - p0 : PREF_TILE, quads = (n + 1) / 2;
     __syncthreads();
-    for (int e = tid; e < 2 * quads; e += PREF_FINISH) {  // an odd number of pairs is filled up with one that is none
+    for (int e = tid; e < 2 * quads; e += threads) {  // an odd number of pairs is filled up with one that is none
       const int c = e < n ? a.chosen[p0 + e] : -1, r = e < n ? a.rejected[p0 + e] : -1;
       const bool ok = c >= 0 && c < a.L && r >= 0 && r < a.L && (!a.weight || a.weight[p0 + e] != 0.f);
       const float s = ok ? a.slope[p0 + e] : 0.f;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs
       slope[2 * e + 1] = -s;
     }
     __syncthreads();
-    for (int e = tid >> 2; e < 2 * n; e += PREF_FINISH / 4) {  // four neighbouring lanes an entry, every fourth quad each
+    for (int e = tid >> 2; e < 2 * n; e += threads / 4) {  // four neighbouring lanes an entry, every fourth quad each
       const int mine = label[e];
       float t = 0.f;
       int first = e;

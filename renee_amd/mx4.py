@@ -23,6 +23,8 @@ class _On:
     """The device of a call: made current where it is not, with its current stream's handle.  (torch.cuda.device and current_stream take
     some 6 us of host time, as much as the smallest of these kernels.)"""
 
+    _ready = set()  # devices whose kernels' limits have been raised: nothing is left to do inside a captured graph
+
     def __init__(self, device: torch.device):
         self.index = device.index
 
@@ -30,6 +32,9 @@ class _On:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
+        if self.index not in _On._ready:
+            check(lib().xfc_init(), "xfc_init")
+            _On._ready.add(self.index)
         return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *_):

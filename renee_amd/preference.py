@@ -18,7 +18,10 @@ labels before the tuning).  Two ways in:
 """
 from __future__ import annotations
 
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
 from .mx4 import MX4Labels, TYPES, _On, _rows
@@ -76,6 +79,7 @@ def preference(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.
     reference = _list(reference, torch.float32, P, device, "reference")
     pair_weight = _list(pair_weight, torch.float32, P, device, "pair_weight")
     _require(0.0 <= label_smoothing <= 1.0, "label_smoothing must be in 0..1", ValueError)
+    _require(math.isfinite(beta), "beta must be finite", ValueError)
     _require(grad_dtype in TYPES, "grad_dtype must be float16, bfloat16 or float32", TypeError)
     if g is not None:
         _require(g.dtype == torch.float16 and g.dim() == 2 and g.device == device and g.shape[0] == bsz and g.shape[1] >= numy and
@@ -113,6 +117,7 @@ class _Preference(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         grad = ctx.grad * grad_out
         return grad if grad.device == ctx.device else grad.to(ctx.device), None, None, None, None, None, None, None, None, None

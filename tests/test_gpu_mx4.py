@@ -119,6 +119,53 @@ def test_a_row_or_label_that_is_no_number_stays_by_itself(dev, bits):
     assert torch.equal(torch.isnan(got), bad)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,scales", [(torch.float16, (6e-8, 3e-7, 1e-5, 1.0, 3e4)), (torch.bfloat16, (1e-38, 3e-38, 1e-5, 1e30)),
+                                          (torch.float32, (1e-43, 1e-40, 2e-38, 1.0, 1e30))])
+def test_embeddings_of_any_size(dev, dtype, scales, bits):
+    """From the smallest numbers of a type to near its largest, each row against labels of one block each."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.cat([torch.randn(7, 96, generator=g) * s for s in scales]).to(dtype)
+    w = torch.zeros(96, 96, dtype=torch.float32)
+    w[torch.arange(96), torch.arange(96)] = 1.0
+    want = O.rounded(x, bits)
+    want[torch.isnan(want).any(1)] = math.nan  # a sum with a NaN is one
+    labels = MX4Labels.from_weight(w.to(dev))
+    v, i = labels.topk(x.to(dev), 8, embed_bits=bits)  # fp32 sums of one number each
+    best = O.topk(want, 8)
+    # A row with an infinity (fp16 at 3e4) has no scores.  Of numbers whose scale times the labels' lies below fp32's normal numbers only
+    # that they stay there is asked.
+    small = want.abs().nan_to_num(1.0).amax(1) < 2.0 ** -118
+    v, i = v.cpu().double(), i.cpu()
+    assert torch.equal(v[~small], best[0][~small]) and torch.equal(i[~small], best[1][~small].where(best[1][~small] >= 0, torch.tensor(95)))
+    assert bool(((v[small] - best[0][small]).abs() <= 2.0 ** -118).all())
+
+
+def test_codes_beyond_32_bits(dev):
+    """12,000,010 labels x 768: 4.9 GB of codes.  The last labels' logits, rows, best places and pairs are those of a matrix of them alone."""
+    from renee_amd import pair_margins
+
+    L, d, tail = 12_000_010, 768, 138
+    units = -(-L // 64)
+    g = torch.Generator(device=dev).manual_seed(3)
+    codes = torch.randint(0, 256, (units, 24 * 1024), generator=g, dtype=torch.uint8, device=dev)
+    scales = torch.full((units, 6 * 256), 120, dtype=torch.uint8, device=dev)
+    scales[-2] = 124  # the best labels are among the last
+    labels = MX4Labels(codes, scales, L, d)
+    few = MX4Labels(codes[-3:].clone(), scales[-3:].clone(), tail, d)
+    x = torch.randn(40, d, generator=g, device=dev)
+    assert (L - tail) % 64 == 0
+    for rows in (1, 40):
+        assert torch.equal(labels.xfc_forward(x[:rows])[:, -tail:], few.xfc_forward(x[:rows]))
+        v, i = labels.topk(x[:rows], 5)
+        ev, ei = few.topk(x[:rows], 5)
+        assert torch.equal(v, ev) and torch.equal(i, ei + L - tail)
+    assert torch.equal(mx4_dequantize(codes[-3:].clone(), scales[-3:].clone(), tail, d), labels.dequantize()[-tail:])
+    rowptr = torch.tensor([0, 3], dtype=torch.int32, device=dev)
+    c, r = (torch.tensor(t, dtype=torch.int32, device=dev) for t in ((0, 70, 137), (137, 5, 64)))
+    assert torch.equal(pair_margins(x[:1], labels, rowptr, c + L - tail, r + L - tail), pair_margins(x[:1], few, rowptr, c, r))
+
+
 # ---- top-K: with 4 bits sums are exact, so that values and labels are those of a stable sort -----------------------------------
 
 @pytest.mark.parametrize("K", [1, 5, 8, 9, 100])

@@ -211,6 +211,80 @@ def test_captured(dev, B, d, most):
         assert all(torch.equal(a, b) for a, b in zip(got, preference(static, labels, rowptr, c, r, ref, wt, 0.9, 0.1)))
 
 
+def test_captured_with_its_backward_pass(dev):
+    x, w = _problem(20, 300, 128, torch.float32, 27)
+    rowptr, c, r, ref, wt = (t.to(dev) for t in _pairs(20, 300, 7, 1))
+    labels = MX4Labels.from_weight(w.to(dev))
+    leaf = x.to(dev).requires_grad_(True)
+
+    def step():
+        preference_loss(leaf, labels, rowptr, c, r, ref, wt, 0.9, 0.1).backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    leaf.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for k in range(3):
+        with torch.no_grad():
+            leaf.copy_(x.to(dev) * (k + 1))
+        leaf.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = preference(leaf.detach(), labels, rowptr, c, r, ref, wt, 0.9, 0.1)[2]
+        assert torch.equal(leaf.grad, want)
+
+
+def test_a_second_derivative_is_refused(dev):
+    x, w = _problem(3, 30, 64, torch.float32, 29)
+    rowptr, c, r, _, _ = (t.to(dev) for t in _pairs(3, 30, 4, 2))
+    leaf = x.to(dev).requires_grad_(True)
+    (grad,) = torch.autograd.grad(preference_loss(leaf, w.to(dev), rowptr, c, r), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+
+
+def test_embeddings_that_are_expanded_strided_or_on_the_cpu(dev):
+    x, w = _problem(6, 50, 64, torch.float32, 33)
+    rowptr, c, r, ref, wt = (t.to(dev) for t in _pairs(6, 50, 6, 4))
+    one = x[:1].to(dev).requires_grad_(True)
+    preference_loss(one.expand(6, 64), w.to(dev), rowptr, c, r, ref, wt, 0.5).backward()
+    want = preference(x[:1].expand(6, 64).to(dev), w.to(dev), rowptr, c, r, ref, wt, 0.5)[2]
+    assert torch.allclose(one.grad, want.sum(0, keepdim=True), rtol=1e-6, atol=1e-6)
+    wide = torch.zeros(6, 130, device=dev)
+    wide[:, 3:67] = x.to(dev)
+    full = preference(x.to(dev), w.to(dev), rowptr, c, r, ref, wt, 0.5)
+    assert all(torch.equal(a, b) for a, b in zip(preference(wide[:, 3:67], w.to(dev), rowptr, c, r, ref, wt, 0.5), full))
+    leaf = x.clone().requires_grad_(True)
+    preference_loss(leaf, w.to(dev), rowptr.cpu(), c.cpu(), r.cpu(), ref.cpu(), wt.cpu(), 0.5).backward()
+    assert leaf.grad.device.type == "cpu" and torch.equal(leaf.grad, full[2].cpu())
+
+
+def test_both_gradients_in_one_call(dev):
+    from renee_amd._lib import check, lib
+
+    x, w = _problem(12, 100, 64, torch.float32, 37)
+    rowptr, c, r, ref, wt = (t.to(dev) for t in _pairs(12, 100, 9, 6))
+    xd, wd = x.to(dev), w.to(dev)
+    want = preference(xd, wd, rowptr, c, r, ref, wt, 0.5)
+    g0 = torch.rand(12, 104, device=dev).half()
+    gw = g0.clone()
+    preference(xd, wd, rowptr, c, r, ref, wt, 0.5, g=gw)
+    P, g = len(c), g0.clone()
+    loss, margin, dx = torch.empty((), device=dev), torch.empty(P, device=dev), torch.full((12, 72), 7.0, device=dev)
+    need = lib().xfc_preference_workspace_bytes(12, P, 64)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    check(lib().xfc_preference(xd.data_ptr(), 2, 64, wd.data_ptr(), 64, None, 100, 64, rowptr.data_ptr(), c.data_ptr(), r.data_ptr(), ref.data_ptr(), wt.data_ptr(),
+                               12, P, 0.5, 0.0, 1.0, loss.data_ptr(), margin.data_ptr(), dx.data_ptr(), 2, 72, g.data_ptr(), 104, ws.data_ptr(), need,
+                               torch.cuda.current_stream().cuda_stream), "xfc_preference")
+    assert torch.equal(loss, want[0]) and torch.equal(margin, want[1]) and torch.equal(dx[:, :64], want[2]) and torch.equal(g, gw)
+    assert bool((dx[:, 64:] == 7).all())
+
+
 def test_on_another_stream(dev):
     x, w = _problem(40, 300, 128, torch.float32, 23)
     rowptr, c, r, ref, wt = (t.to(dev) for t in _pairs(40, 300, 7, 2))
