@@ -136,13 +136,14 @@ int check_product(const void* X, int type, int64_t ldx, const void* codes, const
   return XFC_OK;
 }
 
-// Maxima of a row, as floats.  Up to MX_FINE_ROWS rows a float for each half of a unit, else for each unit, and for K > 8 two halves in its place;
-// whole runs of units, whole pieces of 16 bytes.
-constexpr int64_t MX_FINE_ROWS = 32;
-bool mx_fine(int64_t B, int64_t K) { return K <= TOPK_MAX && B <= MX_FINE_ROWS; }
+// Maxima of a row, as floats: whole runs of units, whole pieces of 16 bytes.  K <= 8: where they are few a float for each half of a unit, from
+// which fewer labels' scores have to be formed again, else for each unit (top-5 of 64 rows x 131,072 x 768 28 us by halves, 32 by units, of
+// 1024 88 and 96; 512 x 320,001 x 384 and more: no difference, and twice the room).  K > 8: two halves in a float's place.
+constexpr int64_t MX_FINE = (int64_t)1 << 27;
+bool mx_fine(int64_t B, int64_t L, int64_t K) { return K <= TOPK_MAX && (B <= 32 || B * L <= MX_FINE); }
 int64_t mx_maxima(int64_t B, int64_t L, int64_t K) {
   const int64_t units = ceil_div(L, MX_UNIT);
-  return round_up(mx_fine(B, K) ? 2 * units : units, 4);
+  return round_up(mx_fine(B, L, K) ? 2 * units : units, 4);
 }
 int64_t mx_half_maxima(int64_t L) { return 2 * (int64_t)ceil_div(L, MX_UNIT); }  // beside logits, halves
 
@@ -262,7 +263,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   }
   float* const bmax = (float*)workspace;
   const int64_t ldb = mx_maxima(B, L, K);
-  const bool fine = mx_fine(B, K);
+  const bool fine = mx_fine(B, L, K);
   const int block = K > TOPK_MAX ? MX_SELECT_BLOCK : fine ? MX_UNIT / 2 : MX_UNIT;
   rc = mx_product(K > TOPK_MAX ? MX_HALF_MAXIMA : MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d,
                   !fine && L >= (1 << 20) ? 4 : 1, fine, st);
