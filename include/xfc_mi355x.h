@@ -312,9 +312,9 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
 /*
  * xfc_topk with an MX4 label matrix: ties to the lower label, labels >= numy returned as numy - 1.  K <= 8: by the fp32 sums; a score that is no number is
  * never selected, and a row with fewer than K others reports (-inf, numy - 1) in the remaining places.  8 < K <= 8192: by the logits of
- * xfc_mx4_logits, a NaN as -inf.  Up to K = 256 of 4096 K labels or more no logits are written either, only maxima of blocks of labels.
- * Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, K); where logits are written and there are more than 256 rows, what 256
- * rows take is enough, the rows then go in turns.
+ * xfc_mx4_logits, a NaN as -inf; up to K = 256 only maxima of blocks of labels are written instead of the logits, where there are enough labels
+ * and rows for it (by a rule that is the library's own).  Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, d, K); where logits are
+ * written (2 L bytes a row and more) and there are more than 256 rows, what 256 rows take is enough, the rows then go in turns.
  */
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t d, int64_t K);
 int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,
@@ -335,7 +335,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
  * X: fp16, bf16 or fp32.  W: fp16 rows, or with scales non-NULL MX4 codes (ldw is not used).  reference, weight, margin, dX, G may be NULL
  * (0, 1, not wanted).  A pair with a label outside [0, L) or weight 0 is not there, whatever else it holds: its margin is 0, and so is
  * that of pairs which no row has.  Row pointers that do not ascend give an unspecified result for the rows of these pairs.  Results do not depend on
- * anything but the arguments: no atomics.  d <= 4096, a multiple of 8; P <= 2^30.
+ * anything but the arguments: no atomics.  d <= 4096, a multiple of 8; P <= 2^30, B <= 2^22 - 2.
  */
 size_t xfc_preference_workspace_bytes(int64_t B, int64_t P, int64_t d);
 int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t ldw, const void* scales, int64_t L, int64_t d,

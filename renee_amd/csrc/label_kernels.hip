@@ -25,6 +25,9 @@ int by_type(int type, Fn&& f) {
   return f(std::integral_constant<int, XFC_F16>{});
 }
 
+// A launch has fewer than 2^32 threads: matrices go in ranges of units, selections in ranges of rows.
+constexpr int64_t MX_GRID = ((int64_t)1 << 24) - 1, SELECT_ROWS = (int64_t)1 << 21;
+
 int check_mx(const void* W, int type, int64_t ldw, int64_t L, int64_t d, const void* codes, const void* scales, bool& empty) {
   empty = false;
   if (!dims_ok(L) || !dims_ok(d) || !type_ok(type)) return XFC_ERR_INVALID;
@@ -32,7 +35,24 @@ int check_mx(const void* W, int type, int64_t ldw, int64_t L, int64_t d, const v
   if (d == 0 || !W || !codes || !scales) return XFC_ERR_INVALID;
   if (d % 8 || !rows_ok(W, type, ldw) || !aligned16(codes) || !aligned16(scales)) return XFC_ERR_ALIGN;
   if (ldw < d) return XFC_ERR_SHAPE;
-  if (ceil_div(L, MX_UNIT) * (int64_t)mx_steps(d) > 0x7fffffff) return XFC_ERR_INVALID;
+  if (mx_steps(d) > MX_GRID) return XFC_ERR_LIMIT;
+  return XFC_OK;
+}
+
+template <class Launch>
+int by_units(const MxArgs& all, int type, Launch&& launch) {
+  const int64_t units = MX_GRID / all.steps;
+  for (int64_t l0 = 0; l0 < all.L; l0 += units * MX_UNIT) {
+    MxArgs a = all;
+    const int64_t u0 = l0 / MX_UNIT, bytes = l0 * a.ldw * type_bytes(type);
+    a.W = a.W ? reinterpret_cast<const char*>(a.W) + bytes : nullptr;
+    a.out = a.out ? reinterpret_cast<char*>(a.out) + bytes : nullptr;
+    a.codes += u0 * mx_code_bytes(a.d);
+    a.scales += u0 * mx_scale_bytes(a.d);
+    a.L = all.L - l0 < units * MX_UNIT ? all.L - l0 : units * MX_UNIT;
+    const int rc = launch(dim3((unsigned)(ceil_div(a.L, MX_UNIT) * (int64_t)a.steps)), a);
+    if (rc) return rc;
+  }
   return XFC_OK;
 }
 
@@ -190,8 +210,11 @@ int xfc_mx4_quantize(const void* W, int type, int64_t ldw, int64_t L, int64_t d,
   const int rc = check_mx(W, type, ldw, L, d, codes, scales, empty);
   if (rc || empty) return rc;
   const MxArgs a = {W, nullptr, ldw, (uint8_t*)codes, (uint8_t*)scales, L, (int)d, mx_blocks(d), mx_steps(d)};
-  const dim3 g((unsigned)(ceil_div(L, MX_UNIT) * (int64_t)a.steps));
-  return by_type(type, [&](auto t) { return launch_k<mx4_quantize_kernel<decltype(t)::value>>(g, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a); });
+  return by_type(type, [&](auto t) {
+    return by_units(a, type, [&](dim3 g, const MxArgs& part) {
+      return launch_k<mx4_quantize_kernel<decltype(t)::value>>(g, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), part);
+    });
+  });
 }
 
 int xfc_mx4_dequantize(const void* codes, const void* scales, int64_t L, int64_t d, void* W, int type, int64_t ldw, void* stream) {
@@ -199,8 +222,11 @@ int xfc_mx4_dequantize(const void* codes, const void* scales, int64_t L, int64_t
   const int rc = check_mx(W, type, ldw, L, d, codes, scales, empty);
   if (rc || empty) return rc;
   const MxArgs a = {nullptr, W, ldw, (uint8_t*)const_cast<void*>(codes), (uint8_t*)const_cast<void*>(scales), L, (int)d, mx_blocks(d), mx_steps(d)};
-  const dim3 g((unsigned)(ceil_div(L, MX_UNIT) * (int64_t)a.steps));
-  return by_type(type, [&](auto t) { return launch_k<mx4_dequantize_kernel<decltype(t)::value>>(g, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a); });
+  return by_type(type, [&](auto t) {
+    return by_units(a, type, [&](dim3 g, const MxArgs& part) {
+      return launch_k<mx4_dequantize_kernel<decltype(t)::value>>(g, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), part);
+    });
+  });
 }
 
 int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, const void* scales, void* out, int64_t ldo,
@@ -248,6 +274,7 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
     const int64_t ldb = mx_half_maxima(L);
     int64_t block = B;
     if (workspace_bytes < need) block = (int64_t)(workspace_bytes / turn) * 256;
+    if (block > SELECT_ROWS) block = SELECT_ROWS;
     const int64_t ldl = round_up(L, MX_UNIT);
     for (int64_t r0 = 0; r0 < B; r0 += block) {
       const int64_t rows = B - r0 < block ? B - r0 : block;
@@ -268,23 +295,28 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   rc = mx_product(K > TOPK_MAX ? MX_HALF_MAXIMA : MX_MAXIMA, x8, X, type, ldx, codes, scales, nullptr, 0, nullptr, bmax, ldb, B, L, d,
                   !fine && L >= (1 << 20) ? 4 : 1, fine, st);
   if (rc) return rc;
-  PickArgs k = {};
-  k.bmax = bmax; k.ldb = ldb; k.n_blocks = ceil_div(L, block); k.N = (int)L; k.K = (int)d; k.topk = K;
-  k.begin = k.end = 1; k.numy = numy; k.out_v = values; k.out_i = indices;
-  auto pick = [&](auto s) {
+  auto pick = [&](auto s, int64_t r0, int64_t rows) {
     using S = decltype(s);
+    PickArgs k = {};
+    k.bmax = bmax + r0 * ldb; k.ldb = ldb; k.n_blocks = ceil_div(L, block); k.N = (int)L; k.K = (int)d; k.topk = K;
+    k.begin = k.end = 1; k.numy = numy; k.out_v = values + r0 * K; k.out_i = indices + r0 * K;
     if (K > TOPK_MAX) {
       constexpr auto kernel = mx4_select_kernel<std::is_same_v<S, MxScores<true>>>;
       if (raise_lds_limit<kernel>(MX_SELECT_LDS) != hipSuccess) return (int)XFC_ERR_HIP;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)B), dim3(MX_SELECT_THREADS), (unsigned)(S::lds(d) + sizeof(MxSelectLds)), st, k, s);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(MX_SELECT_THREADS), (unsigned)(S::lds(d) + sizeof(MxSelectLds)), st, k, s);
       return check_launch();
     }
-    if (fine) hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT / 2, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);  // 11 KB at most
-    else hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)B), dim3(512), (unsigned)S::lds(d), st, k, s);
+    if (fine) hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT / 2, S>), dim3((unsigned)rows), dim3(512), (unsigned)S::lds(d), st, k, s);  // 11 KB at most
+    else hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)rows), dim3(512), (unsigned)S::lds(d), st, k, s);
     return check_launch();
   };
-  if (x8) return pick(MxScores<true>{X, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales});
-  return pick(MxScores<false>{X, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales});
+  for (int64_t r0 = 0; r0 < B && !rc; r0 += SELECT_ROWS) {
+    const int64_t rows = B - r0 < SELECT_ROWS ? B - r0 : SELECT_ROWS;
+    const void* const x = reinterpret_cast<const char*>(X) + r0 * ldx * type_bytes(type);
+    rc = x8 ? pick(MxScores<true>{x, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales}, r0, rows)
+            : pick(MxScores<false>{x, type, ldx, (const uint8_t*)codes, (const uint8_t*)scales}, r0, rows);
+  }
+  return rc;
 }
 
 // Pairs of a wave: as many as a lane each holds, fewer where they would leave the chip's waves without any.  (65,536 pairs of 1024 rows x 768,
@@ -305,7 +337,7 @@ int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t 
                    int64_t B, int64_t P, float beta, float smoothing, float scale, float* loss, float* margin,
                    void* dX, int dx_type, int64_t lddx, void* G, int64_t ldg, void* workspace, size_t workspace_bytes, void* stream) {
   if (!dims_ok(B) || !dims_ok(L) || !dims_ok(d) || !dims_ok(P) || !type_ok(type) || (dX && !type_ok(dx_type))) return XFC_ERR_INVALID;
-  if (!loss || (B > 0 && (!X || !W || !rowptr)) || (P > 0 && (!chosen || !rejected)) || d <= 0 || L <= 0 || B > 0x7fffff) return XFC_ERR_INVALID;
+  if (!loss || (B > 0 && (!X || !W || !rowptr)) || (P > 0 && (!chosen || !rejected)) || d <= 0 || L <= 0 || B > 0x3ffffe) return XFC_ERR_INVALID;  // (threads of a launch)
   if (!(fabsf(beta) <= 3.4e38f) || !(smoothing >= 0.f && smoothing <= 1.f)) return XFC_ERR_INVALID;
   if (B > 0 && (d % 8 || !rows_ok(X, type, ldx) || !aligned16(W) || (scales ? !aligned16(scales) : ldw % 8 != 0) ||
                 (dX && !rows_ok(dX, dx_type, lddx)))) return XFC_ERR_ALIGN;

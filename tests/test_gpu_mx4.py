@@ -166,6 +166,30 @@ def test_codes_beyond_32_bits(dev):
     assert torch.equal(pair_margins(x[:1], labels, rowptr, c + L - tail, r + L - tail), pair_margins(x[:1], few, rowptr, c, r))
 
 
+def test_matrices_of_more_than_one_launch(dev):
+    """A launch has fewer than 2^24 workgroups of 256 threads: units behind those come out as in a matrix of them alone."""
+    units, d, tail = (1 << 24) + 5, 8, 7 * 64 - 30
+    L = units * 64 - 30
+    w = torch.empty(L, d, dtype=torch.float16, device=dev).fill_(0.5)
+    w[-tail:] = _matrix(tail, d, torch.float16, 9).to(dev)
+    codes, scales = mx4_quantize(w)
+    ec, es = mx4_quantize(w[-tail:].clone())
+    assert torch.equal(codes[-7:], ec) and torch.equal(scales[-7:], es)
+    assert torch.equal(codes[:-7], codes[:1].expand(units - 7, -1)) and torch.equal(scales[:-7], scales[:1].expand(units - 7, -1))
+    assert torch.equal(mx4_dequantize(codes, scales, L, d)[-tail:], mx4_dequantize(ec, es, tail, d))
+
+
+@pytest.mark.parametrize("K", [3, 12])
+def test_topk_of_more_rows_than_a_launch_has(dev, K):
+    x, w, _ = _problem(1000, 64, 8, 4, torch.float16, 12)
+    labels = MX4Labels.from_weight(w.to(dev))
+    B = (1 << 22) + 100
+    many = x.to(dev).repeat(B // 1000 + 1, 1)[:B]
+    v, i = labels.topk(many, K)
+    ev, ei = labels.topk(x.to(dev), K)
+    assert torch.equal(v, ev.repeat(B // 1000 + 1, 1)[:B]) and torch.equal(i, ei.repeat(B // 1000 + 1, 1)[:B])
+
+
 # ---- top-K: with 4 bits sums are exact, so that values and labels are those of a stable sort -----------------------------------
 
 @pytest.mark.parametrize("K", [1, 5, 8, 9, 100])

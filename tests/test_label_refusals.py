@@ -18,7 +18,7 @@ def _quantize(W=ONE, type=F16, ldw=64, L=10, d=64, codes=ONE, scales=ONE):
 @pytest.mark.parametrize("how,code", [
     (dict(W=None), 1), (dict(codes=None), 1), (dict(scales=None), 1), (dict(type=3), 1), (dict(L=-1), 1), (dict(d=0), 1), (dict(L=1 << 31), 1),
     (dict(d=60), 3), (dict(ldw=68), 3), (dict(type=F32, ldw=66), 3), (dict(W=ctypes.c_void_p(24)), 3), (dict(codes=ctypes.c_void_p(8)), 3),
-    (dict(ldw=56), 6), (dict(L=0, W=None, codes=None, scales=None), 0)])
+    (dict(ldw=56), 6), (dict(L=0, W=None, codes=None, scales=None), 0), (dict(d=(1 << 31) - 8, ldw=(1 << 31) - 8), 7)])
 def test_quantize(how, code):
     assert _quantize(**how) == code
     if "codes" not in how or how["codes"] is not None:
@@ -68,7 +68,7 @@ def _preference(X=ONE, type=F16, ldx=64, W=ONE, ldw=64, scales=None, L=10, d=64,
 
 @pytest.mark.parametrize("how,code", [
     (dict(X=None), 1), (dict(W=None), 1), (dict(rowptr=None), 1), (dict(chosen=None), 1), (dict(rejected=None), 1), (dict(loss=None), 1), (dict(L=0), 1),
-    (dict(d=0), 1), (dict(P=-1), 1), (dict(B=1 << 23), 1), (dict(dx_type=7), 1), (dict(smoothing=1.5), 1), (dict(smoothing=float("nan")), 1), (dict(beta=float("nan")), 1), (dict(beta=float("inf")), 1),
+    (dict(d=0), 1), (dict(P=-1), 1), (dict(B=1 << 23), 1), (dict(B=(1 << 22) - 1), 1), (dict(dx_type=7), 1), (dict(smoothing=1.5), 1), (dict(smoothing=float("nan")), 1), (dict(beta=float("nan")), 1), (dict(beta=float("inf")), 1),
     (dict(ldx=60), 3), (dict(ldw=60), 3), (dict(scales=ctypes.c_void_p(8)), 3), (dict(ldx=56), 6), (dict(ldw=56), 6), (dict(lddx=56), 6), (dict(G=ONE, ldg=9), 6),
     (dict(d=4104, ldx=4104, ldw=4104, lddx=4104), 7), (dict(P=(1 << 30) + 1), 7), (dict(dX=ctypes.c_void_p(8)), 3), (dict(lddx=66), 3), (dict(ws=None), 4), (dict(nbytes=16), 4), (dict(ws=ctypes.c_void_p(24)), 3)])
 def test_preference(how, code):
