@@ -189,8 +189,10 @@ int xfc::init_labels() {
   both(std::integral_constant<int, MX_LOGITS_MAX>{});
   both(std::integral_constant<int, MX_MAXIMA>{});
   both(std::integral_constant<int, MX_HALF_MAXIMA>{});
-  keep(raise_lds_limit<mx4_select_kernel<true>>(MX_SELECT_LDS));
-  keep(raise_lds_limit<mx4_select_kernel<false>>(MX_SELECT_LDS));
+  keep(raise_lds_limit<mx4_select_kernel<true, 512>>(MX_SELECT_LDS));
+  keep(raise_lds_limit<mx4_select_kernel<true, 1024>>(MX_SELECT_LDS));
+  keep(raise_lds_limit<mx4_select_kernel<false, 512>>(MX_SELECT_LDS));
+  keep(raise_lds_limit<mx4_select_kernel<false, 1024>>(MX_SELECT_LDS));
   return e == hipSuccess ? XFC_OK : XFC_ERR_HIP;
 }
 
@@ -301,10 +303,15 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
     k.bmax = bmax + r0 * ldb; k.ldb = ldb; k.n_blocks = ceil_div(L, block); k.N = (int)L; k.K = (int)d; k.topk = K;
     k.begin = k.end = 1; k.numy = numy; k.out_v = values + r0 * K; k.out_i = indices + r0 * K;
     if (K > TOPK_MAX) {
-      constexpr auto kernel = mx4_select_kernel<std::is_same_v<S, MxScores<true>>>;
-      if (raise_lds_limit<kernel>(MX_SELECT_LDS) != hipSuccess) return (int)XFC_ERR_HIP;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(MX_SELECT_THREADS), (unsigned)(S::lds(d) + sizeof(MxSelectLds)), st, k, s);
-      return check_launch();
+      auto select = [&](auto threads) {
+        constexpr int T = decltype(threads)::value;
+        constexpr auto kernel = mx4_select_kernel<std::is_same_v<S, MxScores<true>>, T>;
+        if (raise_lds_limit<kernel>(MX_SELECT_LDS) != hipSuccess) return (int)XFC_ERR_HIP;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(T), (unsigned)(S::lds(d) + sizeof(MxSelectLds)), st, k, s);
+        return check_launch();
+      };
+      if (rows > num_cus()) return select(std::integral_constant<int, 512>{});
+      return select(std::integral_constant<int, 1024>{});
     }
     if (fine) hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT / 2, S>), dim3((unsigned)rows), dim3(512), (unsigned)S::lds(d), st, k, s);  // 11 KB at most
     else hipLaunchKernelGGL((topk_pick_kernel<MX_UNIT, S>), dim3((unsigned)rows), dim3(512), (unsigned)S::lds(d), st, k, s);

@@ -696,18 +696,25 @@ struct MxScores {
 // One workgroup per row.  The K-th largest of the threads' own largest maxima, to eleven bits, is no larger than the K-th maximum; the blocks that
 // reach it, a few more than K, are listed and ranked by comparing each with all.  Only if there is no room for them (rows of many
 // equal scores) are the maxima counted by their upper eleven bits and then, in the bin that the K-th is in, by the lower five, and of those
-// at the K-th key the first ones taken.  Sixteen waves then form the scores, a block at a time each.  Bound by fetching K x 32 labels
-// a row, after some 25 us for the blocks: 512 rows x 40,960 blocks, K = 100, 668 MB of codes and scales, 145 to 152 us.  (Blocks of 16 would halve that, but their maxima cost the product more than they
-// save.)
-constexpr int MX_SELECT_K = 256, MX_SELECT_BLOCK = 32, MX_SELECT_THREADS = 1024, MX_SELECT_BINS = 2048;
+// at the K-th key the first ones taken.  The waves then form the scores, a block at a time each.  Bound by fetching K x 32 labels
+// a row, after some 25 us for the blocks: 512 rows x 40,960 blocks, K = 100, 668 MB of codes and scales, 136 us.  (Blocks of 16 would halve that, but
+// their maxima cost the product more than they save; blocks in the order of labels, for the rows to share fetches, 137 us.)
+//
+// More rows than the chip has CUs: two workgroups of 512 threads to a CU, one finds its blocks while the other fetches; else one of 1024.  (K = 100, us by
+// 512 / by 1024, with the product: 512 rows x 1,310,720 x 768 363 / 373, 300 292 / 305, 256 239 / 216, 32 209 / 174; 512 x 320,001 x 64 53 / 62.)
+constexpr int MX_SELECT_K = 256, MX_SELECT_BLOCK = 32, MX_SELECT_LIST = 512, MX_SELECT_BINS = 2048;
 
 // (of PickArgs: bmax, two halves a float; n_blocks; N, K, topk, numy, out_v, out_i)
 struct MxSelectLds {
-  unsigned long long cand[MX_SELECT_K * MX_SELECT_BLOCK];
-  int hist[MX_SELECT_BINS];
+  union {
+    unsigned long long cand[MX_SELECT_K * MX_SELECT_BLOCK];
+    struct {  // before there are any
+      int hist[MX_SELECT_BINS];
+      unsigned long long list[MX_SELECT_LIST];
+    };
+  };
   int block[MX_SELECT_K];
-  unsigned long long list[MX_SELECT_THREADS];
-  int wave_tot[MX_SELECT_THREADS / 64];
+  int wave_tot[16];
   int bin, above, n_block, n_cand;
 };
 
@@ -721,15 +728,15 @@ __device__ __forceinline__ float half_unkey(uint32_t k) {
   return (float)__builtin_bit_cast(half_t, h);
 }
 
-template <bool X8>
-__global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs a, MxScores<X8> scores) {
+template <bool X8, int THREADS>
+__global__ void __launch_bounds__(THREADS) mx4_select_kernel(PickArgs a, MxScores<X8> scores) {
   MxSelectLds& S = *reinterpret_cast<MxSelectLds*>(MxScores<X8>::room() + MxScores<X8>::lds(a.K));  // a multiple of 16
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int K = a.topk;  // there are more blocks
   const uint32_t* const maxima = reinterpret_cast<const uint32_t*>(a.bmax) + (int64_t)row * a.ldb;  // two blocks each
   const int quads = (a.n_blocks + 7) / 8;
   auto for_each = [&](auto&& f) {
-    for (int w = tid; w < quads; w += MX_SELECT_THREADS) {
+    for (int w = tid; w < quads; w += THREADS) {
       const uint4v v = *reinterpret_cast<const uint4v*>(maxima + 4 * w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -765,7 +772,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
   };
   // The same by counting all maxima; leaves the blocks and returns the K-th key.
   auto by_counts = [&]() -> uint32_t {
-    for (int i = tid; i < MX_SELECT_BINS; i += MX_SELECT_THREADS) S.hist[i] = 0;
+    for (int i = tid; i < MX_SELECT_BINS; i += THREADS) S.hist[i] = 0;
     if (tid == 0) S.n_block = 0;
     __syncthreads();
     for_each([&](uint32_t key, int) { atomicAdd(&S.hist[key >> 5], 1); });
@@ -782,7 +789,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
     const int at_least = K - S.above;  // blocks at the K-th key that are taken, the first ones
     // (the list's order is of no matter)
     int taken = 0;
-    for (int w0 = 0; w0 < quads; w0 += MX_SELECT_THREADS) {
+    for (int w0 = 0; w0 < quads; w0 += THREADS) {
       uint32_t here = 0, equal = 0;  // of this thread's eight blocks: above the key, at it
       if (w0 + tid < quads) {
         const uint4v v = *reinterpret_cast<const uint4v*>(maxima + 4 * (w0 + tid));
@@ -807,7 +814,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
         if (lane == 63) S.wave_tot[wave] = rank;
         __syncthreads();
         int before = taken, all = 0;
-        for (int w = 0; w < MX_SELECT_THREADS / 64; ++w) {
+        for (int w = 0; w < THREADS / 64; ++w) {
           before += w < wave ? S.wave_tot[w] : 0;
           all += S.wave_tot[w];
         }
@@ -820,7 +827,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
     }
     return least;
   };
-  for (int i = tid; i < MX_SELECT_BINS; i += MX_SELECT_THREADS) S.hist[i] = 0;
+  for (int i = tid; i < MX_SELECT_BINS; i += THREADS) S.hist[i] = 0;
   if (tid == 0) S.n_block = S.n_cand = 0;
   scores.open(a, row);
   uint32_t largest = 0;
@@ -833,13 +840,13 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
   for_each([&](uint32_t key, int block) {
     if (key < bound) return;
     const int at = atomicAdd(&S.n_block, 1);
-    if (at < MX_SELECT_THREADS) S.list[at] = ((unsigned long long)key << 32) | (uint32_t)~block;
+    if (at < MX_SELECT_LIST) S.list[at] = ((unsigned long long)key << 32) | (uint32_t)~block;
   });
   __syncthreads();
   const int listed = S.n_block;
   __syncthreads();
   uint32_t least;
-  if (listed <= MX_SELECT_THREADS) {
+  if (listed <= MX_SELECT_LIST) {
     if (tid < listed) {
       const unsigned long long mine = S.list[tid];
       int rank = 0;
@@ -853,7 +860,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
     least = by_counts();
   }
   const int n_block = K;
-  for (int u = wave; u < n_block; u += MX_SELECT_THREADS / 64) {
+  for (int u = wave; u < n_block; u += THREADS / 64) {
     const int block = __builtin_amdgcn_readfirstlane(S.block[u]) * MX_SELECT_BLOCK;
     const int first[2] = {block, block + 16};
     float4v z[2];
@@ -877,7 +884,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
     a.out_i[(int64_t)row * K + at] = label < a.numy ? label : a.numy - 1;
   };
   const int n = S.n_cand;
-  if (n <= MX_SELECT_THREADS) {
+  if (n <= THREADS) {
     if (tid < n) {
       const unsigned long long mine = S.cand[tid];
       int rank = 0;
@@ -889,11 +896,11 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
   // bitonic over the next power of two
   int size = 64;
   while (size < n) size <<= 1;
-  for (int i = n + tid; i < size; i += MX_SELECT_THREADS) S.cand[i] = 0;
+  for (int i = n + tid; i < size; i += THREADS) S.cand[i] = 0;
   __syncthreads();
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = tid; i < size; i += MX_SELECT_THREADS) {
+      for (int i = tid; i < size; i += THREADS) {
         const int o = i ^ j;
         if (o > i) {
           const unsigned long long x = S.cand[i], y = S.cand[o];
@@ -902,7 +909,7 @@ __global__ void __launch_bounds__(MX_SELECT_THREADS) mx4_select_kernel(PickArgs 
       }
       __syncthreads();
     }
-  for (int i = tid; i < K; i += MX_SELECT_THREADS) write(i, S.cand[i]);
+  for (int i = tid; i < K; i += THREADS) write(i, S.cand[i]);
 }
 
 }  // namespace xfc

@@ -202,9 +202,9 @@ def test_topk_with_4_bits(dev, B, L, d, K):
     assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
 
 
-# (above 8 by maxima alone from 32 rows and 1000 K or more labels on, here 36, 130 and 33 rows)
+# (above 8 by maxima alone from 32 rows and 1000 K or more labels on, here 36, 130, 33 and 300 rows: those that several at a time share a CU)
 @pytest.mark.parametrize("B,L,d,K", [(2, 70001, 64, 5), (40, 66000, 128, 100), (5, 140003, 64, 8), (3, 70001, 64, 3000), (36, 18729, 8, 9), (130, 40961, 72, 10),
-                                     (33, 70001, 200, 16), (3, 414001, 64, 100), (34, 600003, 8, 256), (130, 270011, 8, 256)])
+                                     (33, 70001, 200, 16), (3, 414001, 64, 100), (34, 600003, 8, 256), (130, 270011, 8, 256), (300, 41000, 200, 20)])
 def test_topk_of_many_labels(dev, B, L, d, K):
     x, w, z = _problem(B, L, d, 4, torch.float16, L + K)
     v, i = MX4Labels.from_weight(w.to(dev)).topk(x.to(dev), K, embed_bits=4)
@@ -240,14 +240,14 @@ def test_topk_ties_go_to_the_lower_label_and_constant_rows(dev):
 
 
 @pytest.mark.parametrize("K", [9, 12])
-@pytest.mark.parametrize("L", [1000, 32003])
-def test_topk_above_8_counts_nan_as_the_least(dev, L, K):
+@pytest.mark.parametrize("B,L", [(40, 1000), (40, 32003), (300, 16003)])
+def test_topk_above_8_counts_nan_as_the_least(dev, B, L, K):
     """Rows of equal scores, of fewer numbers than K, of none, and of infinities."""
     w = torch.zeros(L, 64, dtype=torch.float16)
     w[:, 0] = torch.randint(-2, 3, (L,), generator=torch.Generator().manual_seed(L)).half()
     w[5::3] = float("nan")
     w[:, 40] = torch.where(torch.arange(L) % 1009 == 7, 6.0e4, 0.0).half()
-    x = torch.zeros(40, 64, dtype=torch.float32)  # by maxima with 32,003 labels
+    x = torch.zeros(B, 64, dtype=torch.float32)  # by maxima with 16,003 and 32,003 labels
     x[5:, 2] = 1.0
     x[0, 0], x[1, 1], x[2, 0], x[3, 40], x[4, 40] = 1.0, 1.0, float("nan"), 1e30, -1e30
     some = w.clone()
