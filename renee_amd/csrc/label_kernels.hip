@@ -122,6 +122,35 @@ int launch_product(int out, bool x8, const MxPlan& p, const MxProductArgs& a, hi
   return launch_product<false, MX_MAXIMA>(p, a, st);
 }
 
+// Maxima by mx4_wide_kernel: rows that fill its tiles as well as those of 128, and units enough to a workgroup to make up for its rows' quantisation.
+// (Time of top-5 with mx4_product_kernel over that with it.  Units to a workgroup 16: 400 rows x 262,144 labels x 768 0.95, 512 1.01; 18: 400 x 300,001 x 512 1.00, x 384 1.01; 32:
+// 512 x 524,288 x 768 1.04, 1000 x 262,144 1.03; 80: 512 x 1,310,720 x 768 1.11, x 256 1.09; 160 and more 1.12 to 1.39.  Rows that fill fewer tiles of 128: 768 x 700,001 x 768
+// 0.98, 640 0.88.)
+bool mx_wide(int64_t rows, int64_t units, int steps, int cus) {
+  const int64_t tiles = ceil_div(rows, MX_WIDE_ROWS);
+  return steps >= 2 && steps <= 6 && round_up(rows, MX_WIDE_ROWS) == round_up(rows, 128) && units * tiles >= (int64_t)20 * cus;
+}
+template <int STEPS, int OUT>
+int launch_wide(const MxProductArgs& args, int cus, hipStream_t st) {
+  MxProductArgs a = args;
+  const int per_xcd = cus / 8 > 0 ? cus / 8 : 1, most = ceil_div(ceil_div(a.units, MxSection<STEPS>::UNITS), 8);
+  a.tiles_m = ceil_div(a.M, MX_WIDE_ROWS);
+  a.slots = per_xcd / a.tiles_m;
+  if (a.slots > most) a.slots = most;
+  if (a.slots < 1) a.slots = 1;
+  return launch_lds<mx4_wide_kernel<STEPS, OUT>>(dim3((unsigned)(8 * a.slots * a.tiles_m)), dim3(64 * MX_WAVES), MxSection<STEPS>::SLOTS * MxSection<STEPS>::BYTES, st, a);
+}
+template <int OUT>
+int launch_wide(const MxProductArgs& a, int cus, hipStream_t st) {
+  switch (a.steps) {
+    case 2: return launch_wide<2, OUT>(a, cus, st);
+    case 3: return launch_wide<3, OUT>(a, cus, st);
+    case 4: return launch_wide<4, OUT>(a, cus, st);
+    case 5: return launch_wide<5, OUT>(a, cus, st);
+    default: return launch_wide<6, OUT>(a, cus, st);
+  }
+}
+
 // Rows of one launch: the row tiles of an XCD's workgroups.
 constexpr int64_t MX_ROWS = 2048;
 
@@ -140,6 +169,11 @@ int mx_product(int out, bool x8, const void* X, int type, int64_t ldx, const voi
     a.M = (int)rows; a.N = (int)L; a.K = (int)d;
     a.units = ceil_div(L, MX_UNIT); a.blocks = mx_blocks(d); a.steps = mx_steps(d);
     a.tiles_m = p.tiles_m; a.slots = p.slots; a.run = run; a.fine = fine;
+    if (!x8 && !fine && (out == MX_MAXIMA || out == MX_HALF_MAXIMA) && mx_wide(rows, a.units, a.steps, num_cus())) {
+      const int rc = out == MX_MAXIMA ? launch_wide<MX_MAXIMA>(a, num_cus(), st) : launch_wide<MX_HALF_MAXIMA>(a, num_cus(), st);
+      if (rc) return rc;
+      continue;
+    }
     const int rc = launch_product(out, x8, p, a, st);
     if (rc) return rc;
   }
@@ -189,6 +223,16 @@ int xfc::init_labels() {
   both(std::integral_constant<int, MX_LOGITS_MAX>{});
   both(std::integral_constant<int, MX_MAXIMA>{});
   both(std::integral_constant<int, MX_HALF_MAXIMA>{});
+  auto wide = [&](auto out) {
+    constexpr int OUT = decltype(out)::value;
+    keep(raise_lds_limit<mx4_wide_kernel<2, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_wide_kernel<3, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_wide_kernel<4, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_wide_kernel<5, OUT>>(FULL_LDS));
+    keep(raise_lds_limit<mx4_wide_kernel<6, OUT>>(FULL_LDS));
+  };
+  wide(std::integral_constant<int, MX_MAXIMA>{});
+  wide(std::integral_constant<int, MX_HALF_MAXIMA>{});
   keep(raise_lds_limit<mx4_select_kernel<true, 512>>(MX_SELECT_LDS));
   keep(raise_lds_limit<mx4_select_kernel<true, 1024>>(MX_SELECT_LDS));
   keep(raise_lds_limit<mx4_select_kernel<false, 512>>(MX_SELECT_LDS));

@@ -361,10 +361,49 @@ __device__ __forceinline__ void store_first(half_t* to, const half8& h, int n) {
   }
 }
 
+// The largest of a lane's eight labels of half p of a unit, for its row of row tile j.
+template <int NT>
+__device__ __forceinline__ float mx_largest(const float4v (&acc)[MX_TILES][NT], int j, int p) {
+  const float4v lo = acc[2 * p][j < NT ? j : NT - 1], hi = acc[2 * p + 1][j < NT ? j : NT - 1];
+  return max3_num(max3_num(lo[0], lo[1], lo[2]), lo[3], max3_num(hi[0], hi[1], max_num(hi[2], hi[3])));
+}
+// ... over the four lanes that have the row: of four row tiles, lane group g ends up with tile 4 n + g.
+template <class Of>
+__device__ __forceinline__ float mx_over_lanes(int n, Of&& of) {
+  return fold16(fold32(of(4 * n), of(4 * n + 2)), fold32(of(4 * n + 1), of(4 * n + 3)));
+}
+// Both halves' maxima as logits, in a float's place; no number is -inf.
+template <int NT>
+__device__ __forceinline__ float mx_half_maxima(const float4v (&acc)[MX_TILES][NT], int n) {
+  typedef half_t half2v __attribute__((ext_vector_type(2)));
+  const float least = -__builtin_huge_valf();
+  const half2v two = {(half_t)max_num(mx_over_lanes(n, [&](int j) { return mx_largest(acc, j, 0); }), least),
+                      (half_t)max_num(mx_over_lanes(n, [&](int j) { return mx_largest(acc, j, 1); }), least)};
+  return __builtin_bit_cast(float, two);
+}
+// The maxima above are inline asm, in front of which the compiler puts no wait states: the last MFMAs' results are waited for here.  Labels behind the last
+// are made no numbers.
+template <int NT>
+__device__ __forceinline__ void mx_before_maxima(float4v (&acc)[MX_TILES][NT], int label0, int labels, int q) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15");
+  __builtin_amdgcn_sched_barrier(0);
+  if (label0 + MX_UNIT > labels) {
+#pragma unroll
+    for (int t = 0; t < MX_TILES; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool in = label0 + mx_label(t, 4 * q + r) < labels;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[t][j][r] = in ? acc[t][j][r] : __builtin_nanf("");
+      }
+  }
+}
+
 // Bound, with few rows, by the stream of codes: 16 rows x 131,072 x 768 12.8 us for 54 MB of them and 4 of logits, 4.5 TB/s.  With many, logits
 // by the memory that they go to (512 x 1,310,720: 1.34 GB of them beside 0.53 of codes, 455 us at best, 530 to 590 with a warm chip), maxima by the
-// matrix pipes' power: 1024 x 2,812,281 x 768 with 4-bit rows takes 990 to 1,080 us, 4.1 to 4.5 PFLOP/s at a clock that falls to 1.7 GHz (registers alone
-// reach 7 PFLOP/s on random numbers, 9.6 on zeros); without the fetches it would be 200 us less, without the maxima 90.
+// matrix pipes' power: 1024 x 2,812,281 x 768 with 4-bit rows took 990 to 1,080 us, 4.1 to 4.5 PFLOP/s at a clock that falls to 1.7 GHz (registers alone
+// reach 7 PFLOP/s on random numbers, 9.6 on zeros); without the fetches it was 200 us less, without the maxima 90: mx4_wide_kernel has such calls now.
 //
 // A workgroup keeps its rows' fragments in the LDS and its waves, which never meet again, stream units of 64 labels past them, straight
 // into the A side's registers: two steps on their way, across units.  (Three or six took as long where there is much to do, and longer where
@@ -479,31 +518,11 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     const int label0 = unit * MX_UNIT;
     const bool edge = label0 + MX_UNIT > a.N;
     if constexpr (OUT == MX_MAXIMA || OUT == MX_HALF_MAXIMA) {
-      // The maxima below are inline asm, in front of which the compiler puts no wait states: the last MFMAs' results are waited for here.
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_nop 15\n\ts_nop 15");
-      __builtin_amdgcn_sched_barrier(0);
-      if (edge) {
-#pragma unroll
-        for (int t = 0; t < MX_TILES; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool in = label0 + mx_label(t, 4 * q + r) < a.N;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[t][j][r] = in ? acc[t][j][r] : __builtin_nanf("");
-          }
-      }
-      // of this lane's eight labels of half p
-      auto largest = [&](int j, int p) {
-        const float4v lo = acc[2 * p][j < NT ? j : NT - 1], hi = acc[2 * p + 1][j < NT ? j : NT - 1];
-        return max3_num(max3_num(lo[0], lo[1], lo[2]), lo[3], max3_num(hi[0], hi[1], max_num(hi[2], hi[3])));
-      };
-      // lane group g ends up with row tile 4 n + g
-      auto over_lanes = [&](int n, auto of) { return fold16(fold32(of(4 * n), of(4 * n + 2)), fold32(of(4 * n + 1), of(4 * n + 3))); };
+      mx_before_maxima(acc, label0, a.N, q);
       if (OUT == MX_MAXIMA && a.fine) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          const float m0 = over_lanes(n, [&](int j) { return largest(j, 0); }), m1 = over_lanes(n, [&](int j) { return largest(j, 1); });
+          const float m0 = mx_over_lanes(n, [&](int j) { return mx_largest(acc, j, 0); }), m1 = mx_over_lanes(n, [&](int j) { return mx_largest(acc, j, 1); });
           const int row = row0 + 64 * n + lane_now;
           if (4 * n + q < NT && row < a.M) *reinterpret_cast<float2v*>(a.bmax + (int64_t)row * a.ldb + 2 * (int64_t)unit) = float2v{m0, m1};
         }
@@ -512,15 +531,8 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           float m;
-          if constexpr (OUT == MX_MAXIMA) {
-            m = over_lanes(n, [&](int j) { return max_num(largest(j, 0), largest(j, 1)); });
-          } else {
-            typedef half_t half2v __attribute__((ext_vector_type(2)));
-            const float least = -__builtin_huge_valf();
-            const half2v two = {(half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 0); }), least),
-                                (half_t)max_num(over_lanes(n, [&](int j) { return largest(j, 1); }), least)};
-            m = __builtin_bit_cast(float, two);
-          }
+          if constexpr (OUT == MX_MAXIMA) m = mx_over_lanes(n, [&](int j) { return max_num(mx_largest(acc, j, 0), mx_largest(acc, j, 1)); });
+          else m = mx_half_maxima(acc, n);
 #pragma unroll
           for (int r = 0; r < 4; ++r) best[n][r] = r4 == r ? m : best[n][r];
         }
@@ -605,6 +617,157 @@ __global__ void __launch_bounds__(64 * MX_WAVES, NT >= 4 ? 2 : 4) mx4_product_ke
     turn(slot[0]);
     turn(slot[1]);
   }
+}
+
+// Maxima of many rows of 4 bits and many labels: the rows stay in registers, 64 of them a wave for as long as the kernel runs, and the codes are streamed through
+// the LDS, two units at a time (a section) that all eight waves multiply with: 512 rows a workgroup where the kernel above has 128, so that a quarter of the codes
+// cross from the L2s, for as many bytes out of the LDS.  (1024 x 2,812,281 x 768 1,071 -> 958 us, 512 x 1,310,720 282 -> 260; the first 13 of them
+// quantise rows, which is why there have to be many labels.  With 8 bits, 256 rows a workgroup, 1.00 to 1.05 of the kernel above; logits 564 -> 730, whose rows
+// are written in shorter pieces.)
+template <int STEPS>
+struct MxSection {
+  static constexpr int UNITS = 2, CODES = UNITS * STEPS * 4096, SCALES = (UNITS * STEPS * 256 + 1023) / 1024 * 1024, BYTES = CODES + SCALES;
+  static constexpr int SLOTS = 3;      // one in use, two on their way
+  static constexpr int FETCHES = STEPS + 1;  // of a wave
+  static_assert(SLOTS * BYTES <= 160 * 1024, "LDS");
+};
+constexpr int MX_WIDE_TILES = 4, MX_WIDE_ROWS = MX_WAVES * 16 * MX_WIDE_TILES;
+
+// f(0) ... f(N - 1), as constants: what indexes registers has to be written out, which the compiler leaves off with loops of that size.
+template <int N, class Fn>
+__device__ __forceinline__ void written_out(Fn&& f) {
+  [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
+}
+
+template <int STEPS, int OUT>
+__global__ void __launch_bounds__(64 * MX_WAVES) mx4_wide_kernel(MxProductArgs a) {
+  using Rows = MxRows<false>;
+  using Section = MxSection<STEPS>;
+  constexpr int NR = MX_WIDE_TILES;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+  const int row0 = ((local % a.tiles_m) * MX_WAVES + wave) * 16 * NR;
+  const int workers = 8 * a.slots, worker = xcd * a.slots + local / a.tiles_m;
+  const int sections = (a.units + Section::UNITS - 1) / Section::UNITS;
+  const int64_t unit_codes = mx_code_bytes(a.K), unit_scales = mx_scale_bytes(a.K);
+
+  // A section's tiles lie in the LDS as lanes read them, one after the other, whatever the width (of a block that is none any other).  Past the last
+  // section that one is fetched again, so that as many fetches are on their way as ever; of a unit that is none, the one before.
+  const int whole = a.blocks >> 2, wide = a.blocks & 3;  // steps of four blocks, blocks of the step behind them
+  const uint32_t at_whole = (uint32_t)(4 * i + q) * 16, at_rest = (uint32_t)(wide * i + (q < wide ? q : wide - 1)) * 16;
+  auto fetch = [&](int section, int slot) __attribute__((always_inline)) {
+    const int sec = section < sections ? section : sections - 1;
+    const int units = a.units - sec * Section::UNITS < Section::UNITS ? a.units - sec * Section::UNITS : Section::UNITS;
+    unsigned char* const to = smem_raw + slot * Section::BYTES;
+    const uint8_t* const c = a.codes + (int64_t)sec * Section::UNITS * unit_codes;
+    const uint8_t* const s = a.scales + (int64_t)sec * Section::UNITS * unit_scales;
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {  // tiles, dealt to the waves
+      const int at = (wave >> 2) + 2 * n, u = at >= STEPS && units > 1 ? 1 : 0, step = at >= STEPS ? at - STEPS : at, tile = wave & 3;
+      const bool rest = step >= whole;
+      load16_to_lds(c + u * unit_codes + (rest ? whole * 4096 + tile * wide * 256 : step * 4096 + tile * 1024), rest ? at_rest : at_whole,
+                    to + (wave + MX_WAVES * n) * 1024);
+    }
+    // (waves that have no part of the scales fetch the first once more)
+    const uint32_t part = wave * 1024 < Section::SCALES ? wave * 1024 : 0, at = part + lane * 16, last = (uint32_t)(units * unit_scales) - 16;
+    load16_to_lds(s, at < last ? at : last, to + Section::CODES + part);
+  };
+  fetch(worker, 0);
+
+  // The wave's rows, quantised as in the kernel above, a tile at a time through its part of the other slots.
+  int8v rows[STEPS][NR];
+  uint32_t row_scales[STEPS] = {};
+  constexpr int ROOM = (Section::SLOTS - 1) * Section::BYTES / MX_WAVES / 16 * 16;
+  static_assert(ROOM >= STEPS * (Rows::FRAG + 64), "room for a tile");
+  unsigned char* const stage = smem_raw + Section::BYTES + wave * ROOM;
+  unsigned char* const stage_scales = stage + STEPS * Rows::FRAG;
+  auto lds_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+  auto fill = [&](auto many, auto load) __attribute__((always_inline)) {
+    constexpr int N = decltype(many)::value;  // rows of a lane on their way
+    const int part = lane & 3, block = (lane >> 2) & 3, k = block * MX_BLOCK + part * 8;
+    written_out<NR>([&](auto jt) __attribute__((always_inline)) {
+      constexpr int j = decltype(jt)::value;
+#pragma unroll
+      for (int r0 = lane >> 4; r0 < 16; r0 += 4 * N) {
+        decltype(load((int64_t)0)) v[N][STEPS];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int row = row0 + 16 * j + r0 + 4 * n;
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) {
+            v[n][s] = {};
+            if (row < a.M && s * MX_STEP + k < a.K) v[n][s] = load((int64_t)row * a.ldx + s * MX_STEP + k);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) {
+            const uint32_t byte = Rows::put(stage + s * Rows::FRAG, v[n][s], r0 + 4 * n, block, part);
+            if (part == 0) stage_scales[s * 64 + block * 16 + r0 + 4 * n] = (unsigned char)byte;
+          }
+      }
+      lds_done();
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        rows[s][j] = Rows::get(stage + s * Rows::FRAG, lane);
+        row_scales[s] |= (uint32_t)stage_scales[s * 64 + lane] << (8 * j);
+      }
+      lds_done();
+    });
+  };
+  if (a.type == XFC_F16) fill(std::integral_constant<int, 4>{}, [&](int64_t at) { return *reinterpret_cast<const half8*>(reinterpret_cast<const half_t*>(a.X) + at); });
+  else fill(std::integral_constant<int, 1>{}, [&](int64_t at) { return load8_of(a.X, a.type, at); });
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int s = 1; s < Section::SLOTS; ++s) fetch(worker + s * workers, s);
+
+  struct Slot { int4v w[MX_TILES]; uint32_t s; };
+  Slot slot[2];
+  auto read = [&](const unsigned char* c, int u, int step, Slot& to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < MX_TILES; ++t) to.w[t] = *reinterpret_cast<const int4v*>(c + ((u * STEPS + step) * MX_TILES + t) * 1024 + lane * 16);
+    to.s = *reinterpret_cast<const uint32_t*>(c + Section::CODES + u * (int)unit_scales + step * 256 + lane * 4);
+  };
+  float4v acc[MX_TILES][NR];
+  int in = 0;
+  // What this wave has asked for of the first section is there, and after the barrier what all have.
+  wait_vmcnt<(Section::SLOTS - 1) * Section::FETCHES>();
+  asm volatile("s_barrier" ::: "memory");
+  for (int section = worker; section < sections; section += workers) {
+    const unsigned char* const c = smem_raw + in * Section::BYTES;
+    float4v best = {};
+    read(c, 0, 0, slot[0]);
+    written_out<Section::UNITS>([&](auto ut) __attribute__((always_inline)) {
+      constexpr int U = decltype(ut)::value;
+      written_out<STEPS>([&](auto st) __attribute__((always_inline)) {
+        constexpr int STEP = decltype(st)::value, NOW = (U * STEPS + STEP) & 1;
+        if constexpr (STEP + 1 < STEPS) read(c, U, STEP + 1, slot[NOW ^ 1]);
+        else if constexpr (U + 1 < Section::UNITS) read(c, U + 1, 0, slot[NOW ^ 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        written_out<NR>([&](auto jt) __attribute__((always_inline)) {
+          written_out<MX_TILES>([&](auto tt) __attribute__((always_inline)) {
+            constexpr int J = decltype(jt)::value, T = decltype(tt)::value;
+            acc[T][J] = mx_mfma<false, T, J>(slot[NOW].w[T], slot[NOW].s, rows[STEP][J], row_scales[STEP], STEP == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : acc[T][J]);
+          });
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      mx_before_maxima(acc, (section * Section::UNITS + U) * MX_UNIT, a.N, q);
+      if constexpr (OUT == MX_MAXIMA) best[U] = mx_over_lanes(0, [&](int j) { return max_num(mx_largest(acc, j, 0), mx_largest(acc, j, 1)); });
+      else best[U] = mx_half_maxima(acc, 0);
+    });
+    // The next section is there, and all have read this one.  (Fetches and stores return in order.)
+    wait_vmcnt<(Section::SLOTS - 2) * Section::FETCHES>();
+    asm volatile("s_barrier" ::: "memory");
+    fetch(section + Section::SLOTS * workers, in);
+    in = in + 1 == Section::SLOTS ? 0 : in + 1;
+    const int row = row0 + lane;
+    if (row < a.M) *reinterpret_cast<float2v*>(a.bmax + (int64_t)row * a.ldb + 2 * (int64_t)section) = float2v{best[0], best[1]};
+  }
+  wait_vmcnt<0>();  // of fetches into the LDS that no wave has any more
 }
 
 // The scores of sixteen labels of a row formed again, for topk_pick_kernel and below: any sixteen, each lane of the A side fetches its own.  The

@@ -212,6 +212,28 @@ def test_topk_of_many_labels(dev, B, L, d, K):
     assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
 
 
+# (enough rows and labels for the rows to stay in registers, of one to four row tiles and 2 to 6 steps; of 2,500 rows the last 452 do not)
+@pytest.mark.parametrize("B,L,d,K,dtype", [(450, 330001, 200, 5, torch.float16), (512, 340000, 384, 8, torch.float32), (2500, 90017, 512, 3, torch.bfloat16),
+                                           (1024, 170001, 640, 20, torch.float16), (512, 327745, 768, 8, torch.float16), (900, 164000, 744, 10, torch.float32)])
+def test_topk_of_many_rows_and_labels(dev, B, L, d, K, dtype):
+    g = torch.Generator(device=dev).manual_seed(L)
+    w = (torch.randn(L, d, generator=g, device=dev) * 0.02).half()
+    x = torch.randn(B, d, generator=g, device=dev).to(dtype)
+    w[-1] *= 1.5
+    w[L // 2, 3], w[7, d - 1], x[B - 1, d - 1] = float("nan"), float("inf"), float("nan")
+    labels = MX4Labels.from_weight(w)
+    v, i = labels.topk(x, K, embed_bits=4)
+    exact = labels.dequantize(torch.float32).double().t().contiguous()
+    rows = mx4_dequantize(*mx4_quantize(x), B, d, torch.float32).double()
+    for r0 in range(0, B, 128):
+        z = rows[r0:r0 + 128] @ exact
+        z = torch.where(torch.isnan(z), -math.inf, z.half().double() if K > 8 else z)
+        ev, ei = (t[:, :K] for t in torch.sort(z, dim=1, descending=True, stable=True))
+        assert torch.equal(v[r0:r0 + 128].double(), ev)
+        some = ev > -math.inf  # (up to 8 a row without numbers reports the last label)
+        assert torch.equal(i[r0:r0 + 128][some], ei[some])
+
+
 @pytest.mark.parametrize("B,L,d,K", [(1, 1000, 768, 5), (40, 3001, 200, 8), (140, 2000, 64, 3), (20, 4000, 384, 50)])
 def test_topk_with_8_bits(dev, B, L, d, K):
     """The labels' scores are within the product's tolerance of the definition's, none that was left out is above them by more than
