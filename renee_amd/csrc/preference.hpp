@@ -11,9 +11,9 @@
 // a part of, that part: preference_finish_kernel adds those up.  Everything is summed in fp32 in a fixed order (the loss in double): pairs in
 // their order within a chunk, chunks in theirs.
 //
-// 65,536 pairs of 1024 rows over 1,310,720 fp16 labels x 768: 43 us and 8 behind them (201 MB of rows asked for, a half of which the caches have); 512 rows' pairs into G, 131,072 labels: 11 and
-// 6; 32 rows over MX4 labels: 10 and 4, the latency of a chunk's loads.  (Fetching the next four pairs before these are summed: 42.8 -> 42.3 us, and
-// longer where there are few pairs: not kept.)
+// 65,536 pairs of 1024 rows over 1,310,720 fp16 labels x 768: 26 us and 8 behind them (201 MB of rows asked for, a half of which the caches have; 43 with the
+// functions of a pair in all lanes and differences by conversions, which took as much of the vector units as the sums); 512 rows' pairs into G, 131,072
+// labels: 9.4 and 5.6; 32 rows over MX4 labels: 9.5 and 3.8, the latency of a chunk's loads.
 #pragma once
 #include "mx4.hpp"
 
@@ -49,18 +49,41 @@ __device__ __forceinline__ void pref_range(const PrefArgs& a, int row, int& begi
   end = end < begin ? begin : end;
 }
 
-// Eight dims from k on of a label.
-template <bool MX>
+// Eight dims from k on of a label in MX4.
 __device__ __forceinline__ Float8 pref_load(const PrefArgs& a, int label, int k) {
+  const int blocks = mx_blocks(a.d), within = label % MX_UNIT, tile = mx_tile(within), row = mx_row(within), block = k / MX_BLOCK;
+  const uint8_t* const c = reinterpret_cast<const uint8_t*>(a.W) + label / MX_UNIT * mx_code_bytes(a.d);
+  const uint8_t* const s = a.scales + label / MX_UNIT * mx_scale_bytes(a.d);
+  const uint32_t codes = *reinterpret_cast<const uint32_t*>(c + mx_code_at(tile, row, block, blocks) + (k % MX_BLOCK) / 2);
+  return from_fp4(codes, scale_value(s[mx_scale_at(tile, row, block)]));
+}
+
+// u - v of halves as a float, in one instruction where conversions would be two more.  (LO: the lower ones of two, else the upper ones.)
+template <bool LO>
+__device__ __forceinline__ float pref_minus(uint32_t u, uint32_t v) {
+  float r;
+  if constexpr (LO) asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[1,0,1]" : "=v"(r) : "v"(u), "v"(v));
+  else asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,1] op_sel_hi:[1,0,1]" : "=v"(r) : "v"(u), "v"(v));
+  return r;
+}
+// Eight dims from k on of the difference of two labels.
+template <bool MX>
+__device__ __forceinline__ Float8 pref_difference(const PrefArgs& a, int chosen, int rejected, int k) {
+  Float8 f;
   if constexpr (MX) {
-    const int blocks = mx_blocks(a.d), within = label % MX_UNIT, tile = mx_tile(within), row = mx_row(within), block = k / MX_BLOCK;
-    const uint8_t* const c = reinterpret_cast<const uint8_t*>(a.W) + label / MX_UNIT * mx_code_bytes(a.d);
-    const uint8_t* const s = a.scales + label / MX_UNIT * mx_scale_bytes(a.d);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(c + mx_code_at(tile, row, block, blocks) + (k % MX_BLOCK) / 2);
-    return from_fp4(codes, scale_value(s[mx_scale_at(tile, row, block)]));
+    const Float8 u = pref_load(a, chosen, k), v = pref_load(a, rejected, k);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = u.v[e] - v.v[e];
   } else {
-    return load8<XFC_F16>(reinterpret_cast<const half_t*>(a.W) + (int64_t)label * a.ldw + k);
+    const half_t* const w = reinterpret_cast<const half_t*>(a.W) + k;
+    const uint4v u = *reinterpret_cast<const uint4v*>(w + (int64_t)chosen * a.ldw), v = *reinterpret_cast<const uint4v*>(w + (int64_t)rejected * a.ldw);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f.v[2 * e] = pref_minus<true>(u[e], v[e]);
+      f.v[2 * e + 1] = pref_minus<false>(u[e], v[e]);
+    }
   }
+  return f;
 }
 
 // The wave's sum, uniform: within rows of 16 lanes, then across them.
@@ -140,9 +163,7 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           const int k = 512 * c + 8 * lane;  // (no branches: all of the pairs' loads are on their way together)
-          const Float8 u = pref_load<MX>(a, lc, k < a.d ? k : 0), v = pref_load<MX>(a, lr, k < a.d ? k : 0);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) diff[j][c].v[e] = k < a.d ? u.v[e] - v.v[e] : 0.f;
+          diff[j][c] = pref_difference<MX>(a, lc, lr, k < a.d ? k : 0);
         }
       }
       float z[PAIRS];
@@ -150,25 +171,40 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
       for (int j = 0; j < PAIRS; ++j) {
         z[j] = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
+          float part = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) z[j] = fmaf(x[c].v[e], diff[j][c].v[e], z[j]);
+          for (int e = 0; e < 8; ++e) part = fmaf(x[c].v[e], diff[j][c].v[e], part);
+          z[j] += 512 * c + 8 * lane < a.d ? part : 0.f;
+        }
         z[j] = wave_sum(z[j]);
+      }
+      // The pairs' own lanes, all at once: these functions are as much work as a pair's sums.
+      bool mine = false;
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) {
+        m = lane == at[j] ? z[j] : m;
+        mine = mine || lane == at[j];
+      }
+      m -= ref;
+      const float t = a.beta * m, small = expf(-fabsf(t)), rest = small / (1.f + small);  // rest: 1 - sigmoid(|t|)
+      // (a positive margin's slope is -(1 - sigmoid) + e: formed so, what is left at sigmoid near 1 keeps its bits)
+      const float g = wt * a.beta * (t >= 0.f ? a.smoothing - rest : rest - (1.f - a.smoothing));
+      const float l = wt * (log1pf(small) + (t >= 0.f ? a.smoothing * t : -(1.f - a.smoothing) * t));
+      if (mine) {
+        my_margin = m;
+        my_slope = g;
+        loss += (double)l;
       }
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         if (j < n) {
-          const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), at[j]));
-          const float m = z[j] - __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ref), at[j])), t = a.beta * m;
-          const float small = expf(-fabsf(t)), sig = t >= 0.f ? 1.f / (1.f + small) : small / (1.f + small);
-          // (a positive margin's slope is -(1 - sigmoid) + e: formed so, what is left at sigmoid near 1 keeps its bits)
-          const float g = w * a.beta * (t >= 0.f ? a.smoothing - small / (1.f + small) : sig - (1.f - a.smoothing));
-          loss += (double)(w * (log1pf(small) + (t >= 0.f ? a.smoothing * t : -(1.f - a.smoothing) * t)));
-          if (lane == at[j]) { my_margin = m; my_slope = g; }
+          const float gj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), at[j]));
 #pragma unroll
           for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[c].v[e] = fmaf(g, diff[j][c].v[e], acc[c].v[e]);
+            for (int e = 0; e < 8; ++e) acc[c].v[e] = fmaf(gj, diff[j][c].v[e], acc[c].v[e]);
         }
       }
     }
@@ -194,6 +230,8 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
     if (a.margin) a.margin[p0 + lane] = my_margin;
     if (a.G) a.slope[p0 + lane] = my_slope;
   }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) loss += __shfl_xor(loss, off, 64);
   if (lane == 0) a.part_loss[chunk] = loss;
 }
 
