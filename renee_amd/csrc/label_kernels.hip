@@ -416,8 +416,16 @@ int xfc_preference(const void* X, int type, int64_t ldx, const void* W, int64_t 
                  : d <= 2048 ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 8>{});
     if (rc) return rc;
   }
-  const bool rows = B > 0 && (G || dX);
-  return launch_k<preference_finish_kernel>(dim3((unsigned)(rows ? B + 1 : 1)), dim3(rows && !G ? 256 : PREF_FINISH), 0, st, a);
+  // Behind them: a workgroup for each row, several where rows are few, as they may be long.
+  const int64_t rows = G || dX ? B : 0, pieces = d / 8;
+  const int threads = G ? PREF_FINISH : PREF_FINISH / 2;
+  a.slices = 1;
+  if (dX) {
+    const int64_t want = rows > 0 ? ceil_div(512, rows) : 1, most = ceil_div(pieces, 8), least = ceil_div(pieces, threads);
+    a.slices = (int)(want > most ? most : want < least ? least : want);
+  }
+  a.width = ceil_div(pieces, a.slices);
+  return launch_k<preference_finish_kernel>(dim3((unsigned)(rows * a.slices + 1)), dim3(threads), 0, st, a);
 }
 
 }  // extern "C"

@@ -11,9 +11,9 @@
 // a part of, that part: preference_finish_kernel adds those up.  Everything is summed in fp32 in a fixed order (the loss in double): pairs in
 // their order within a chunk, chunks in theirs.
 //
-// 65,536 pairs of 1024 rows over 1,310,720 fp16 labels x 768: 26 us and 8 behind them (201 MB of rows asked for, a half of which the caches have; 43 with the
+// 65,536 pairs of 1024 rows over 1,310,720 fp16 labels x 768: 26 us and 5 behind them (201 MB of rows asked for, a half of which the caches have; 43 with the
 // functions of a pair in all lanes and differences by conversions, which took as much of the vector units as the sums); 512 rows' pairs into G, 131,072
-// labels: 9.4 and 5.6; 32 rows over MX4 labels: 9.5 and 3.8, the latency of a chunk's loads.
+// labels: 9.4 and 5.8; 32 rows over MX4 labels: 9.5 and 5, the latency of a chunk's loads.
 #pragma once
 #include "mx4.hpp"
 
@@ -21,8 +21,9 @@ namespace xfc {
 
 constexpr int PREF_WAVES = 4;
 constexpr int pref_pairs(int pieces) { return pieces <= 2 ? 4 : 8 / pieces; }  // as many as the registers hold
-constexpr int PREF_FINISH = 1024;  // threads of a row with G
+constexpr int PREF_FINISH = 1024;  // threads with G, half of them without
 constexpr int PREF_TILE = 512;  // pairs of a row whose entries of G are joined at a time
+constexpr int PREF_COMPARED = 256;  // ... by comparing each with all others: 9 us, as long as sorting any number takes; 512 37
 
 struct PrefArgs {
   const void* X; int type; int64_t ldx;
@@ -32,6 +33,7 @@ struct PrefArgs {
   const float* reference; const float* weight;        // may be null: 0, 1
   int B, P;
   int chunk, chunks;                                   // pairs of a wave; waves
+  int slices, width;                                   // workgroups of a row behind them; of so many pieces of eight dims
   float beta, smoothing, scale;
   float* margin;                                       // may be null
   void* dX; int dx_type; int64_t lddx;                 // may be null
@@ -235,15 +237,53 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
   if (lane == 0) a.part_loss[chunk] = loss;
 }
 
-// What is left after the pairs, a workgroup per row: dX of rows without pairs and of those that several chunks have a part of, and G.
-// A row's entries of G, two a pair, are joined PREF_TILE pairs at a time: each is compared with all others, the first of a label adds up all of them, in an order that
-// their number alone decides, and rounds G once.  Workgroup B sums the loss.
+// More entries of G: sorted by label, a thread each, within a wave by exchanges between lanes.  Sums over equal labels then double in reach step by step (a label that
+// far away is the same only if all between are), and the last entry of a label has its sum.
+__device__ __forceinline__ void pref_join_sorted(const int32_t* label, const float* slope, int entries, float* room, half_t* g) {
+  static_assert(PREF_FINISH == 2 * PREF_TILE, "a thread for each entry");
+  unsigned long long* const keys = reinterpret_cast<unsigned long long*>(room);
+  uint32_t* const sorted = reinterpret_cast<uint32_t*>(keys + PREF_FINISH);
+  float* const sums = reinterpret_cast<float*>(sorted + PREF_FINISH);  // two of them
+  const int i = threadIdx.x;
+  unsigned long long key = i < entries ? ((unsigned long long)(uint32_t)label[i] << 32) | (unsigned)i : ~0ull;  // no label: behind all others
+  for (int k = 2; k <= PREF_FINISH; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      unsigned long long other;
+      if (j < 64) {
+        other = __shfl_xor(key, j, 64);
+      } else {
+        __syncthreads();
+        keys[i] = key;
+        __syncthreads();
+        other = keys[i ^ j];
+      }
+      const bool lower = ((i & k) == 0) == ((i & j) == 0);  // of the two, the smaller one stays
+      key = (other < key) == lower ? other : key;
+    }
+  const uint32_t mine = (uint32_t)(key >> 32);
+  float t = (uint32_t)key < (uint32_t)entries ? slope[(uint32_t)key] : 0.f;
+  sorted[i] = mine;
+  int half = 0;
+  for (int off = 1; off < PREF_FINISH; off <<= 1, half ^= PREF_FINISH) {
+    sums[half + i] = t;
+    __syncthreads();
+    if (i >= off && sorted[i - off] == mine) t += sums[half + i - off];
+  }
+  if (mine < 0x80000000u && (i + 1 == PREF_FINISH || sorted[i + 1] != mine)) g[mine] = (half_t)((float)g[mine] + t);
+}
+
+// What is left after the pairs: dX of rows without pairs and of those that several chunks have a part of, and G.  A workgroup has `width` pieces of eight dims of a row: one
+// thread for each adds up to four parts, more are dealt to all the threads there are and joined through the LDS, in an order that the arguments alone decide.  (8192 pairs
+// of one row x 768, both kernels: 570 us with one thread for each piece and one workgroup for the row, 21.)
+// A row's entries of G, two a pair, are joined PREF_TILE pairs at a time, and G is rounded once for each label.  Of few each is compared with all others, the first of a
+// label adds up all of them; more are sorted.  (64 rows of 1024 pairs, both kernels: 116 us by comparing, 61.)  The last workgroup sums the loss.
 __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs a) {
   __shared__ __attribute__((aligned(16))) int32_t label[2 * PREF_TILE];
   __shared__ __attribute__((aligned(16))) float slope[2 * PREF_TILE];
+  __shared__ __attribute__((aligned(16))) float join[PREF_FINISH * 8];
   __shared__ double sums[PREF_FINISH / 64];
-  const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
-  if (row == (int)gridDim.x - 1) {
+  const int tid = threadIdx.x, threads = blockDim.x;
+  if (blockIdx.x == gridDim.x - 1) {
     double t = 0.0;
     for (int i = tid; i < a.chunks; i += threads) t += a.part_loss[i];
 #pragma unroll
@@ -256,27 +296,50 @@ __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs
     }
     return;
   }
+  const int row = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x % (unsigned)a.slices;
   int begin, end;
   pref_range(a, row, begin, end);
   if (a.dX) {
+    constexpr int AT_ONCE = 4;
     const int first = begin / a.chunk, last = end > begin ? (end - 1) / a.chunk : first;
     if (begin == end || first < last) {
-      for (int k = 8 * tid; k < a.d; k += 8 * threads) {
-        Float8 t = {};
-        if (begin < end) {
-          for (int c = first; c <= last; ++c) {
-            const Float8 part = load8<XFC_F32>(a.part_dx + (2 * (int64_t)c + (c == first ? 1 : 0)) * a.d + k);
+      const int groups = threads / a.width, group = tid / a.width, piece = slice * a.width + tid % a.width, k = 8 * piece;
+      const int parts = begin < end ? last - first + 1 : 0, per = parts <= AT_ONCE ? AT_ONCE : (parts + groups - 1) / groups;
+      Float8 t = {};
+      if (group < groups && k < a.d) {
+        const int until = first + (group + 1) * per < first + parts ? first + (group + 1) * per : first + parts;
+        for (int c0 = first + group * per; c0 < until; c0 += AT_ONCE) {
+          Float8 part[AT_ONCE];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t.v[e] += part.v[e];
+          for (int j = 0; j < AT_ONCE; ++j) {
+            const int c = c0 + j < until ? c0 + j : c0;
+            part[j] = load8<XFC_F32>(a.part_dx + (2 * (int64_t)c + (c == first ? 1 : 0)) * a.d + k);
+          }
+#pragma unroll
+          for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t.v[e] += c0 + j < until ? part[j].v[e] : 0.f;
+        }
+      }
+      if (parts > AT_ONCE) {
+        store8<XFC_F32>(join + 8 * tid, t);
+        __syncthreads();
+        if (group == 0) {
+          for (int g = 1; g < groups; ++g) {
+            const Float8 other = load8<XFC_F32>(join + 8 * (g * a.width + tid));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t.v[e] += other.v[e];
           }
         }
+      }
+      if (group == 0 && k < a.d) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) t.v[e] *= a.scale;
         pref_store(a, (int64_t)row * a.lddx + k, t);
       }
     }
   }
-  if (!a.G) return;
+  if (!a.G || slice) return;
   half_t* const g = a.G + (int64_t)row * a.ldg;
   for (int p0 = begin; p0 < end; p0 += PREF_TILE) {
     const int n = end - p0 < PREF_TILE ? end - p0 : PREF_TILE, quads = (n + 1) / 2;
@@ -291,6 +354,10 @@ __global__ void __launch_bounds__(PREF_FINISH) preference_finish_kernel(PrefArgs
       slope[2 * e + 1] = -s;
     }
     __syncthreads();
+    if (n > PREF_COMPARED) {
+      pref_join_sorted(label, slope, 4 * quads, join, g);
+      continue;
+    }
     for (int e = tid >> 2; e < 2 * n; e += threads / 4) {  // four neighbouring lanes an entry, every fourth quad each
       const int mine = label[e];
       float t = 0.f;

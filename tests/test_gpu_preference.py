@@ -12,12 +12,16 @@ pytestmark = pytest.mark.gpu
 
 
 def _pairs(B, L, most, seed, few=None):
-    """rowptr, chosen, rejected: up to `most` pairs a row, some rows without; labels among the first `few` repeat."""
+    """rowptr, chosen, rejected: up to `most` pairs a row (of two numbers the second is a middle row's), some rows without; labels among the
+    first `few` repeat."""
     g = torch.Generator().manual_seed(seed)
+    most, long = most if isinstance(most, tuple) else (most, None)
     n = torch.randint(0, most + 1, (B,), generator=g)
     n[0::5] = 0
     if B == 1:
         n[0] = most
+    if long is not None:
+        n[B // 2] = long
     rowptr = torch.cat([torch.zeros(1, dtype=torch.long), n.cumsum(0)]).int()
     P = int(rowptr[-1])
     c = torch.randint(0, few or L, (P,), generator=g).int()
@@ -40,7 +44,8 @@ def _check(got, want, scale, steps, what):
 @pytest.mark.parametrize("mx", [False, True])
 @pytest.mark.parametrize("B,L,d,most,dtype", [(1, 2, 8, 1, torch.float32), (1, 50, 64, 700, torch.float32), (5, 100, 200, 3, torch.float16), (33, 1000, 768, 9, torch.float32),
                                               (64, 300, 136, 70, torch.bfloat16), (3, 5000, 1024, 400, torch.float16), (1100, 200, 96, 4, torch.float32),
-                                              (7, 90, 2048, 20, torch.float32), (4, 70, 4096, 9, torch.float16)])
+                                              (7, 90, 2048, 20, torch.float32), (4, 70, 4096, 9, torch.float16), (1, 300, 768, 9000, torch.float32),
+                                              (700, 300, 200, (4, 3000), torch.float16)])
 def test_loss_margins_and_gradient(dev, B, L, d, most, dtype, mx):
     x, w = _problem(B, L, d, dtype, B + d)
     rowptr, c, r, ref, wt = _pairs(B, L, most, L + d)
@@ -116,7 +121,8 @@ def test_masked_pairs_are_not_there(dev):
     assert torch.equal(g0[:, :30].cpu() != 0, want != 0) and bool((g0[:, 30:] == 5).all())
 
 
-@pytest.mark.parametrize("B,L,most,few", [(1, 20, 1, None), (9, 500, 30, 2), (40, 64, 200, 1), (2, 3000, 1500, 3), (300, 1000, 8, None)])
+@pytest.mark.parametrize("B,L,most,few", [(1, 20, 1, None), (9, 500, 30, 2), (40, 64, 200, 1), (2, 3000, 1500, 3), (300, 1000, 8, None),
+                                            (3, 70, 513, None), (1, 2000, 1024, None)])
 def test_pairs_added_to_g(dev, B, L, most, few):
     x, w = _problem(B, L, 64, torch.float16, B + L)
     rowptr, c, r, ref, wt = _pairs(B, L, most, B, few)
