@@ -307,6 +307,35 @@ def test_topk_rows_in_turns(dev):
     assert torch.equal(ei.cpu(), O.topk(z.half().double(), 20)[1])
 
 
+def test_replays_with_rows_in_registers(dev):
+    """Many rows and labels (both forms of maxima), replayed beside eager calls of other labels and beside each other."""
+    L, d, B = 340000, 256, 512
+    g = torch.Generator(device=dev).manual_seed(6)
+    labels, other = (MX4Labels.from_weight((torch.randn(L, d, generator=g, device=dev) * 0.02).half()) for _ in range(2))
+    x = torch.randn(B, d, generator=g, device=dev).half()
+    calls = [lambda m, K=K: m.topk(x, K, embed_bits=4) for K in (5, 40)]
+    graphs, got = [], []
+    for call in calls:
+        call(labels)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(call(labels))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        x.copy_(torch.randn(B, d, generator=g, device=dev).half())
+        want = [call(labels) for call in calls]
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        beside = calls[0](other)
+        torch.cuda.synchronize()
+        for out, w in zip(got, want):
+            assert torch.equal(out[0], w[0]) and torch.equal(out[1], w[1])
+        assert all(torch.equal(p, q) for p, q in zip(beside, calls[0](other)))
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("K", [5, 30])
 def test_replays_of_two_graphs_on_two_streams(dev, bits, K):
