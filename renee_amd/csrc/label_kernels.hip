@@ -199,7 +199,8 @@ int64_t mx_maxima(int64_t B, int64_t L, int64_t K) {
   const int64_t units = ceil_div(L, MX_UNIT);
   return round_up(mx_fine(B, L, K) ? 2 * units : units, 4);
 }
-int64_t mx_half_maxima(int64_t L) { return 2 * (int64_t)ceil_div(L, MX_UNIT); }  // beside logits, halves
+// Beside logits, halves; rows of whole 16-byte pieces, which select_rows reads.
+int64_t mx_half_maxima(int64_t L) { return round_up(2 * (int64_t)ceil_div(L, MX_UNIT), 8); }
 
 // What mx4_select_kernel takes at most: its own, and the row's numbers at 16,384 dims (8 bits: 9,088).
 constexpr int MX_SELECT_LDS = 96 * 1024;

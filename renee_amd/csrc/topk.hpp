@@ -19,7 +19,7 @@ namespace xfc {
 constexpr int TOPK_MAX = 8;
 constexpr int SEL_MAX_K = 8192;
 // Above TOPK_MAX (xfc_kernels.hip): the K largest of each row of fp16 logits, by the maxima of the rows' blocks of LOGIT_BLOCK where
-// bmax is given, which is of use where the first says so.
+// bmax is given, which is of use where the first says so.  ldl and ldb are multiples of 8, and rows have room for a whole last piece of 8.
 __attribute__((visibility("hidden"))) bool select_takes_maxima(int64_t K, int64_t n_blocks);
 __attribute__((visibility("hidden"))) int select_rows(const _Float16* logits, int64_t ldl, int rows, int L, int64_t numy, int K, const _Float16* bmax,
                                                       int64_t ldb, float* values, int64_t* indices, hipStream_t st);

@@ -1717,6 +1717,7 @@ bool xfc::select_takes_maxima(int64_t K, int64_t n_blocks) {
 }
 int xfc::select_rows(const half_t* logits, int64_t ldl, int rows, int L, int64_t numy, int K, const half_t* bmax, int64_t ldb,
                      float* values, int64_t* indices, hipStream_t st) {
+  if (ldl % 8 || (bmax && (ldb % 8 || !aligned16(bmax)))) return XFC_ERR_ALIGN;  // rows are read in 16-byte pieces, the last one whole
   // sample every stride-th 16 KB block first when that still holds 16 K elements and points at about a
   // thousand candidates at most (half the sort buffer)
   const int cap = K <= SEL_SMALL_MAX_K ? SEL_CAP_SMALL : SEL_CAP_LARGE;
