@@ -290,7 +290,7 @@ size_t xfc_layer_workspace_bytes(int64_t max_batch, int64_t L, int64_t d, int64_
  *           32 p + 8 q + 4 t + r of the unit (p, t < 2, q, r < 4)
  *   scales: xfc_mx4_scale_bytes(L, d) bytes, [unit][step][block 4][row 16][tile 4]; those of no block have to be 0
  * Both 16-byte aligned.  The labels behind the last are written as zeros.  W: `type` elements, rows of d with leading dimension ldw; d a multiple of 8,
- * rows 16-byte aligned.
+ * rows 16-byte aligned; XFC_ERR_LIMIT above 2^31 - 128 dims.
  */
 enum xfc_type { XFC_F16 = 0, XFC_BF16 = 1, XFC_F32 = 2 };
 size_t xfc_mx4_code_bytes(int64_t L, int64_t d);

@@ -21,35 +21,16 @@
 #include <type_traits>
 #include <utility>
 
+#include "mx4_layout.hpp"
 #include "pipe_core.hpp"
 #include "topk.hpp"
 
 namespace xfc {
 
-constexpr int MX_BLOCK = 32, MX_UNIT = 64, MX_STEP = 128;  // dims of a block, labels of a unit, dims of a step
-constexpr int MX_TILES = MX_UNIT / 16;
 constexpr uint32_t MX_NAN = 255;
 
 typedef int int4v __attribute__((ext_vector_type(4)));
 typedef int int8v __attribute__((ext_vector_type(8)));
-
-__host__ __device__ inline int mx_blocks(int64_t d) { return (int)((d + MX_BLOCK - 1) / MX_BLOCK); }
-__host__ __device__ inline int mx_steps(int64_t d) { return (int)((d + MX_STEP - 1) / MX_STEP); }
-// bytes of a unit
-__host__ __device__ inline int64_t mx_code_bytes(int64_t d) { return (int64_t)MX_UNIT * MX_BLOCK / 2 * mx_blocks(d); }
-__host__ __device__ inline int64_t mx_scale_bytes(int64_t d) { return (int64_t)MX_UNIT * 4 * mx_steps(d); }
-
-// The label of a unit that row i of tile t is, and back.
-__host__ __device__ inline int mx_label(int t, int i) { return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3); }
-__host__ __device__ inline int mx_tile(int label) { return 2 * (label >> 5) + ((label >> 2) & 1); }
-__host__ __device__ inline int mx_row(int label) { return 4 * ((label >> 3) & 3) + (label & 3); }
-
-// Where in its unit a label's block stands: codes (16 bytes), scale.
-__host__ __device__ inline int mx_code_at(int tile, int row, int block, int blocks) {
-  const int step = block >> 2, wide = blocks - 4 * step < 4 ? blocks - 4 * step : 4;
-  return step * 4096 + ((tile * 16 + row) * wide + (block & 3)) * 16;
-}
-__host__ __device__ inline int mx_scale_at(int tile, int row, int block) { return (block >> 2) * 256 + (block & 3) * 64 + row * 4 + tile; }
 
 // ---------------------------------------------------------------------------------------------
 // blocks
@@ -221,7 +202,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(MxArgs a) {
   const int step = blockIdx.x % (unsigned)a.steps;
   const int lane = threadIdx.x & 63, row = 4 * (threadIdx.x >> 6) + (lane >> 4), block = (lane >> 2) & 3, part = lane & 3;
   const int k = step * MX_STEP + block * MX_BLOCK + part * 8;
-  const int wide = a.blocks - 4 * step < 4 ? a.blocks - 4 * step : 4;
+  const int wide = mx_wide(step, a.blocks);
   Float8 f[MX_TILES];
 #pragma unroll
   for (int t = 0; t < MX_TILES; ++t) {
@@ -230,7 +211,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(MxArgs a) {
     if (label < a.L && k < a.d) f[t] = load8<TYPE>(reinterpret_cast<const char*>(a.W) + (label * a.ldw + k) * type_bytes(TYPE));
   }
   uint32_t bytes = 0;
-  uint8_t* const codes = a.codes + unit * mx_code_bytes(a.d) + step * 4096;
+  uint8_t* const codes = a.codes + unit * mx_code_bytes(a.d) + mx_step_codes(step);
 #pragma unroll
   for (int t = 0; t < MX_TILES; ++t) {
     float by;
@@ -238,7 +219,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(MxArgs a) {
     bytes |= byte << (8 * t);
     if (block < wide) *reinterpret_cast<uint32_t*>(codes + ((t * 16 + row) * wide + block) * 16 + part * 4) = to_fp4(f[t], by);
   }
-  if (part == 0) *reinterpret_cast<uint32_t*>(a.scales + unit * mx_scale_bytes(a.d) + step * 256 + block * 64 + row * 4) = bytes;
+  if (part == 0) *reinterpret_cast<uint32_t*>(a.scales + unit * mx_scale_bytes(a.d) + mx_step_scales(step) + block * 64 + row * 4) = bytes;
 }
 
 template <int TYPE>
@@ -247,10 +228,10 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(MxArgs a) {
   const int step = blockIdx.x % (unsigned)a.steps;
   const int lane = threadIdx.x & 63, row = 4 * (threadIdx.x >> 6) + (lane >> 4), block = (lane >> 2) & 3, part = lane & 3;
   const int k = step * MX_STEP + block * MX_BLOCK + part * 8;
-  const int wide = a.blocks - 4 * step < 4 ? a.blocks - 4 * step : 4;
+  const int wide = mx_wide(step, a.blocks);
   if (block >= wide || k >= a.d) return;
-  const uint32_t bytes = *reinterpret_cast<const uint32_t*>(a.scales + unit * mx_scale_bytes(a.d) + step * 256 + block * 64 + row * 4);
-  const uint8_t* const codes = a.codes + unit * mx_code_bytes(a.d) + step * 4096;
+  const uint32_t bytes = *reinterpret_cast<const uint32_t*>(a.scales + unit * mx_scale_bytes(a.d) + mx_step_scales(step) + block * 64 + row * 4);
+  const uint8_t* const codes = a.codes + unit * mx_code_bytes(a.d) + mx_step_codes(step);
 #pragma unroll
   for (int t = 0; t < MX_TILES; ++t) {
     const int64_t label = unit * MX_UNIT + mx_label(t, row);

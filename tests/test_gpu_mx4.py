@@ -387,3 +387,15 @@ def test_empty_calls(dev):
     none = MX4Labels.from_weight(torch.empty(0, 64, device=dev))
     assert none.xfc_forward(torch.ones(3, 64, device=dev)).shape == (3, 0)
     assert none.dequantize().shape == (0, 64)
+
+
+def test_codes_of_a_label_beyond_32_bits(dev):
+    """One label of 2^26 + 136 dims: its last steps' codes, 2 GiB behind its first ones, are those of these dims alone."""
+    first, d = 1 << 26, (1 << 26) + 136
+    w = torch.full((1, d), 0.5, dtype=torch.float16, device=dev)
+    w[:, first:] = _matrix(1, 136, torch.float16, 17).to(dev)
+    codes, scales = mx4_quantize(w)
+    ec, es = mx4_quantize(w[:, first:].contiguous())
+    assert torch.equal(codes[:, first // 128 * 4096:], ec) and torch.equal(scales[:, first // 128 * 256:], es)
+    back = mx4_dequantize(codes, scales, 1, d)
+    assert torch.equal(back[:, first:], mx4_dequantize(ec, es, 1, 136)) and bool((back[:, :first] == 0.5).all())
