@@ -111,22 +111,26 @@ def pair_margins(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torc
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, embed, labels, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing, scale):
-        loss, _, ctx.grad = preference(embed, labels, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing, scale,
-                                       grad_dtype=embed.dtype, need_grad=ctx.needs_input_grad[0], need_margin=False)
-        ctx.device = embed.device
+        loss, _, grad = preference(embed, labels, rowptr, chosen, rejected, reference, pair_weight, beta, label_smoothing, scale,
+                                   need_grad=ctx.needs_input_grad[0], need_margin=False)
+        ctx.embed_dtype, ctx.embed_device = embed.dtype, embed.device
+        ctx.save_for_backward(grad)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        grad = ctx.grad * grad_out
-        return grad if grad.device == ctx.device else grad.to(ctx.device), None, None, None, None, None, None, None, None, None
+        # Kept in fp32 and rounded once, behind the factor: a loss scale is there to keep what a narrower type would lose before it.
+        (grad,) = ctx.saved_tensors
+        out = torch.mul(grad, grad_out, out=torch.empty_like(grad, dtype=ctx.embed_dtype))
+        return out.to(ctx.embed_device), None, None, None, None, None, None, None, None, None
 
 
 def preference_loss(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: torch.Tensor, rejected: torch.Tensor,
                     reference: torch.Tensor | None = None, pair_weight: torch.Tensor | None = None, beta: float = 0.1,
                     label_smoothing: float = 0.0, scale: float = 1.0) -> torch.Tensor:
-    """The loss as a differentiable scalar: backward() sends scale times its gradient into embed's graph.  `labels` (an XFCLayer, an
+    """The loss as a differentiable scalar: backward() sends scale times its gradient into embed's graph, kept in float32 and rounded
+    to embed's type once, behind the factor that comes down the graph (a gradient scaler's, say).  `labels` (an XFCLayer, an
     MX4Labels or a float16 matrix) are not trained by it; XFCLayer.preference_grad does that."""
     return _Preference.apply(embed, labels, rowptr, chosen, rejected, reference, pair_weight, float(beta), float(label_smoothing),
                              float(scale))
