@@ -131,6 +131,12 @@ def preference_loss(embed: torch.Tensor, labels, rowptr: torch.Tensor, chosen: t
                     label_smoothing: float = 0.0, scale: float = 1.0) -> torch.Tensor:
     """The loss as a differentiable scalar: backward() sends scale times its gradient into embed's graph, kept in float32 and rounded
     to embed's type once, behind the factor that comes down the graph (a gradient scaler's, say).  `labels` (an XFCLayer, an
-    MX4Labels or a float16 matrix) are not trained by it; XFCLayer.preference_grad does that."""
+    MX4Labels or a float16 matrix) are not trained by it, whether or not a matrix requires grad; XFCLayer.preference_grad does that.
+    reference and pair_weight are numbers of the pairs: either is refused if it requires grad."""
+    if torch.is_grad_enabled():
+        for t, what in ((reference, "reference"), (pair_weight, "pair_weight")):
+            _require(not (isinstance(t, torch.Tensor) and t.requires_grad), f"{what} gets no gradient: pass {what}.detach()")
+    if isinstance(labels, torch.Tensor):
+        labels = labels.detach()
     return _Preference.apply(embed, labels, rowptr, chosen, rejected, reference, pair_weight, float(beta), float(label_smoothing),
                              float(scale))

@@ -63,3 +63,12 @@ def test_the_gradient_is_a_saved_tensor(dev):
     again.backward(retain_graph=True)
     again.backward()
     assert torch.equal(leaf.grad, 2 * preference(x.to(dev), w.to(dev), rowptr, c, r)[2].half())
+
+
+def test_a_label_matrix_that_requires_grad_gets_none(dev):
+    x, w = _problem(5, 40, 64, torch.float32, 45)
+    rowptr, c, r = (t.to(dev) for t in _pairs(5, 40, 4, 46)[:3])
+    leaf, labels = x.to(dev).requires_grad_(True), w.to(dev).requires_grad_(True)
+    preference_loss(leaf, labels, rowptr, c, r).backward()
+    assert labels.grad is None and torch.equal(leaf.grad, preference(x.to(dev), w.to(dev), rowptr, c, r)[2])
+    assert not preference_loss(x.to(dev), labels, rowptr, c, r).requires_grad

@@ -95,3 +95,17 @@ def test_python_refuses_what_is_no_gpu_tensor():
         preference(torch.zeros(1, 64), w.float(), i, i, i)
     with pytest.raises(RuntimeError, match="XFCLayer"):
         preference(torch.zeros(1, 64), None, i, i, i)
+
+
+@pytest.mark.parametrize("which", ["reference", "pair_weight"])
+def test_what_gets_no_gradient_may_not_ask_for_one(which):
+    from renee_amd import preference_loss
+
+    i, t = torch.zeros(2, dtype=torch.int32), torch.zeros(2, requires_grad=True)
+    embed, w = torch.zeros(1, 64, requires_grad=True), torch.zeros(10, 64, dtype=torch.float16)
+    for x in (embed, embed.detach()):
+        with pytest.raises(RuntimeError, match=f"{which}.detach"):
+            preference_loss(x, w, i, i, i, **{which: t})
+    for ok in (lambda: preference_loss(embed, w, i, i, i, **{which: t.detach()}), torch.no_grad()(lambda: preference_loss(embed, w, i, i, i, **{which: t}))):
+        with pytest.raises(RuntimeError, match="GPU"):  # refused for nothing but its device
+            ok()
