@@ -121,25 +121,36 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
   const bool in = p0 + lane < p1;
   const int cl = in ? a.chosen[p0 + lane] : -1, rl = in ? a.rejected[p0 + lane] : -1;
   const float ref = in && a.reference ? a.reference[p0 + lane] : 0.f, wt = in && a.weight ? a.weight[p0 + lane] : 1.f;
-  // the row of the first pair: the last one that begins at it or before (B: none)
-  int row = 0;
-  for (int left = a.B; left > 0;) {  // 64 of them looked at at a time
-    const int step = (left + 63) / 64, mid = (lane + 1) * step - 1;
-    const int past = __builtin_popcountll(__ballot(mid < left && a.rowptr[row + (mid < left ? mid : 0) + 1] <= p0));
-    row += past * step;
-    left = left - past * step < step - 1 ? left - past * step : step - 1;
-  }
-  row = __builtin_amdgcn_readfirstlane(row);
+  // The first row from `from` on that ends behind pair p (B: none), of 64 rows looked at at a time.
+  auto search = [&](int from, int p) {
+    for (int left = a.B - from; left > 0;) {
+      const int step = (left + 63) / 64, mid = (lane + 1) * step - 1;
+      const int past = __builtin_popcountll(__ballot(mid < left && a.rowptr[from + (mid < left ? mid : 0) + 1] <= p));
+      from += past * step;
+      left = left - past * step < step - 1 ? left - past * step : step - 1;
+    }
+    return __builtin_amdgcn_readfirstlane(from);
+  };
+  int row = search(0, p0);
   const unsigned long long usable = __ballot(cl >= 0 && cl < a.L && rl >= 0 && rl < a.L && wt != 0.f);
   float my_margin = 0.f, my_slope = 0.f;
   double loss = 0.0;
-  for (int p = p0; p < p1 && row < a.B; ++row) {
+  for (int p = p0; p < p1 && row < a.B;) {
     int begin, end;
     pref_range(a, row, begin, end);
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
+    if (begin >= p1) break;  // nor has any row from here on
     const int first = p > begin ? p : begin, last = end < p1 ? end : p1;  // of the row, in this chunk
-    if (first >= last) continue;
+    if (first >= last) {
+      // None of this row's, and what lies before it is no row's.  The next row that has any is most often near; if not it is searched for: going through
+      // the rows one after the other took 0.14 us for each.
+      p = first;
+      const int next = row + 1 + lane;
+      const unsigned long long near = __ballot(next < a.B && a.rowptr[next + 1] > p);
+      row = near ? row + 1 + __builtin_ctzll(near) : search(row + 1, p);
+      continue;
+    }
     unsigned long long left = usable & (~0ull << (first - p0)) & (~0ull >> (64 - (last - p0)));
     Float8 acc[C];
     Float8 x[C];
@@ -227,6 +238,7 @@ __global__ void __launch_bounds__(64 * PREF_WAVES) preference_kernel(PrefArgs a)
       }
     }
     p = last;
+    ++row;
   }
   if (in) {
     if (a.margin) a.margin[p0 + lane] = my_margin;

@@ -330,3 +330,53 @@ def test_scoring_and_tuning_together(dev):
     values, best = labels.topk(leaf, 5)
     z = labels.xfc_forward(leaf).float()
     assert torch.allclose(values, z.gather(1, best), rtol=2.0 ** -11, atol=1e-6)
+
+
+@pytest.mark.parametrize("empty", ["behind", "before", "between", "no rows"])
+def test_rows_without_pairs_are_not_gone_through(dev, empty):
+    """65,536 rows of which almost none has pairs, and pairs that no row has (a slice of a list's rows): waves go on at the next row that has
+    any, wherever it is.  (Row by row 8.9 ms; 0.13 for all pairs in the first row.)"""
+    B, P = 65536, 1024
+    x, w = _problem(B, 100, 64, torch.float16, 47)
+    g = torch.Generator().manual_seed(1)
+    c, r = (torch.randint(0, 100, (P,), generator=g).int() for _ in range(2))
+    xd, wd, cd, rd = x.to(dev), w.to(dev), c.to(dev), r.to(dev)
+
+    def timed(rowptr):
+        rp, best = rowptr.to(dev), math.inf
+        out = preference(xd, wd, rp, cd, rd)
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            preference(xd, wd, rp, cd, rd)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best, out
+
+    def pointers(*ends):
+        """Of rows that end at these pairs from the given rows on; the first is where row 0 begins."""
+        rp = torch.zeros(B + 1, dtype=torch.int32)
+        for row, pair in ends:
+            rp[row:] = pair
+        return rp
+
+    usual, _ = timed(pointers((0, 0), (1, P)))
+    for rp in {"behind": [pointers((0, 0), (1, 503)), pointers((0, 0), (1, 4))],
+               "before": [pointers((0, 0), (B, P)), pointers((0, 2), (B, P)), pointers((0, 501), (B // 2, 503))],
+               "between": [pointers((0, 0), (1, 2), (B, P)), pointers((0, 1), (3, 2), (70, 3), (40000, 5), (B - 1, 1001), (B, 1022))],
+               "no rows": [pointers((0, P - 4), (1, P)), pointers((0, 500), (1, 503)), pointers((0, P)), pointers((0, 7))]}[empty]:
+        time, got = timed(rp)
+        rows, has, beta = (rp[1:] > rp[:-1]).nonzero().flatten(), torch.zeros(P, dtype=torch.bool), 0.1
+        assert torch.equal((got[2] != 0).any(1).nonzero().flatten().cpu(), rows)
+        for b in rows.tolist():
+            s = slice(int(rp[b]), int(rp[b + 1]))
+            has[s] = True
+            _, margin, _, grad, _ = O.preference(x[b:b + 1], w, torch.tensor([0, s.stop - s.start]), c[s], r[s], beta=beta)
+            # as in test_loss_margins_and_gradient: a lane's eight products, six halvings and the two differences; then the slope and the row's pairs
+            diff = (w.double()[c[s].long()] - w.double()[r[s].long()]).abs()
+            mass = diff @ x[b].double().abs()
+            _check(got[1][s], margin, mass, 16, "margin")
+            _check(got[2][b], grad[0], (beta + beta ** 2 * mass) @ diff, 16 + 8 + s.stop - s.start, "grad_input")
+        assert not got[1].cpu()[~has].any()
+        assert time < 4 * usual
