@@ -313,8 +313,9 @@ int xfc_mx4_logits(const void* X, int type, int64_t ldx, const void* codes, cons
  * xfc_topk with an MX4 label matrix: ties to the lower label, labels >= numy returned as numy - 1.  K <= 8: by the fp32 sums; a score that is no number is
  * never selected, and a row with fewer than K others reports (-inf, numy - 1) in the remaining places.  8 < K <= 8192: by the logits of
  * xfc_mx4_logits, a NaN as -inf; up to K = 256 only maxima of blocks of labels are written instead of the logits, where there are enough labels
- * and rows for it (by a rule that is the library's own).  Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, d, K); where logits are
- * written (2 L bytes a row and more) and there are more than 256 rows, what 256 rows take is enough, the rows then go in turns.
+ * and rows for it (by a rule that is the library's own).  Workspace, 16-byte aligned: xfc_mx4_topk_workspace_bytes(B, L, d, K).  Where logits are
+ * written (2 L bytes a row and more) that is at most 2 GiB or 512 rows' logits, and of more than 256 rows what 256 take is enough: rows that do not fit
+ * go in turns.
  */
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t d, int64_t K);
 int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,

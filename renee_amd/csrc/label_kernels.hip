@@ -300,10 +300,17 @@ static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
   return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_half_maxima(L) * 2 : 0);
 }
 
+// Rows whose logits a call asks for room for: 2 GiB of them, or 512 rows where those are more, whatever the batch.  (Turns of 512 rows / all at once, 768 dims, K =
+// 300: 1024 rows x 1,310,720 labels 1,336 / 1,402 us, 2.8 M 2,715 / 2,949 and 2.8 / 5.7 GB, 600 x 2.8 M 1,760 / 1,755.)
+static int64_t mx_turn_rows(int64_t B, int64_t L, int64_t K) {
+  const int64_t fit = (int64_t)(((size_t)2 << 30) / mx_logit_rows_bytes(256, L, K)) * 256, rows = fit > 512 ? fit : 512;
+  return B < rows ? B : rows;
+}
+
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t d, int64_t K) {
   if (!dims_ok(B) || !dims_ok(L) || !dims_ok(d) || K < 1 || K > SEL_MAX_K || B == 0 || L == 0) return 0;
   if (K <= TOPK_MAX || mx_by_maxima(B, L, d, K)) return (size_t)B * (size_t)mx_maxima(B, L, K) * 4;
-  return mx_logit_rows_bytes(B, L, K);
+  return mx_logit_rows_bytes(mx_turn_rows(B, L, K), L, K);
 }
 
 int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const void* scales, int64_t B, int64_t L, int64_t d,
@@ -312,15 +319,15 @@ int xfc_mx4_topk(const void* X, int type, int64_t ldx, const void* codes, const 
   if (rc || B == 0) return rc;
   if (K < 1 || K > SEL_MAX_K || L < K || numy < 1 || !values || !indices) return XFC_ERR_INVALID;
   const bool maxima = K <= TOPK_MAX || mx_by_maxima(B, L, d, K);
-  const size_t need = xfc_mx4_topk_workspace_bytes(B, L, d, K), turn = mx_logit_rows_bytes(256, L, K);  // all rows, 256 rows' logits
-  if (!workspace || workspace_bytes < (maxima || B <= 256 ? need : turn)) return XFC_ERR_WORKSPACE;
+  const size_t turn = mx_logit_rows_bytes(256, L, K), all = mx_logit_rows_bytes(B, L, K);  // 256 rows' logits, all rows'
+  if (!workspace || workspace_bytes < (maxima ? xfc_mx4_topk_workspace_bytes(B, L, d, K) : B <= 256 ? all : turn)) return XFC_ERR_WORKSPACE;
   if (!aligned16(workspace)) return XFC_ERR_ALIGN;
   const bool x8 = embed_bits == 8;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (!maxima) {
     const int64_t ldb = mx_half_maxima(L);
     int64_t block = B;
-    if (workspace_bytes < need) block = (int64_t)(workspace_bytes / turn) * 256;
+    if (workspace_bytes < all) block = (int64_t)(workspace_bytes / turn) * 256;
     if (block > SELECT_ROWS) block = SELECT_ROWS;
     const int64_t ldl = round_up(L, MX_UNIT);
     for (int64_t r0 = 0; r0 < B; r0 += block) {

@@ -399,3 +399,24 @@ def test_codes_of_a_label_beyond_32_bits(dev):
     assert torch.equal(codes[:, first // 128 * 4096:], ec) and torch.equal(scales[:, first // 128 * 256:], es)
     back = mx4_dequantize(codes, scales, 1, d)
     assert torch.equal(back[:, first:], mx4_dequantize(ec, es, 1, 136)) and bool((back[:, :first] == 0.5).all())
+
+
+def test_topk_of_more_rows_than_the_workspace_has_room_for(dev):
+    """1,600 rows x 700,001 labels, whose logits are more than 2 GiB: in turns of what that holds, as in one workspace for all of them."""
+    from renee_amd._lib import check, lib
+
+    B, L, d, K = 1600, 700001, 64, 300
+    g = torch.Generator(device=dev).manual_seed(8)
+    labels = MX4Labels.from_weight((torch.randn(L, d, generator=g, device=dev) * 0.02).half())
+    x = torch.randn(B, d, generator=g, device=dev).half()
+    need, all_rows = lib().xfc_mx4_topk_workspace_bytes(B, L, d, K), B * (-(-L // 64) * 64 * 2 + (-(-L // 64) * 2 + 7) // 8 * 16)
+    assert need < all_rows and need <= 2 << 30
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    v, i = labels.topk(x, K)
+    assert torch.cuda.max_memory_allocated() - before < need + (64 << 20)
+    ws, ev, ei = torch.empty(all_rows, dtype=torch.uint8, device=dev), torch.empty_like(v), torch.empty_like(i)
+    check(lib().xfc_mx4_topk(x.data_ptr(), 0, d, labels.codes.data_ptr(), labels.scales.data_ptr(), B, L, d, L, K, 8, ev.data_ptr(), ei.data_ptr(), ws.data_ptr(),
+                             all_rows, torch.cuda.current_stream().cuda_stream), "xfc_mx4_topk")
+    assert torch.equal(v, ev) and torch.equal(i, ei)

@@ -109,3 +109,16 @@ def test_what_gets_no_gradient_may_not_ask_for_one(which):
     for ok in (lambda: preference_loss(embed, w, i, i, i, **{which: t.detach()}), torch.no_grad()(lambda: preference_loss(embed, w, i, i, i, **{which: t}))):
         with pytest.raises(RuntimeError, match="GPU"):  # refused for nothing but its device
             ok()
+
+
+def test_the_logits_of_any_batch_take_bounded_workspace():
+    """What top-K above 8 asks for where it writes logits: all rows up to 512 of them or 2 GiB, no more for more rows, and never less for them."""
+    need = lib().xfc_mx4_topk_workspace_bytes
+    per = -(-2812281 // 64) * 64 * 2
+    assert need(512, 2812281, 768, 1000) > 512 * per and need(8192, 2812281, 768, 1000) == need(512, 2812281, 768, 1000) < 3 << 30
+    assert need(100000, 131072, 768, 300) <= 2 << 30 and need(2000, 131072, 768, 300) > 2000 * 131072 * 2
+    for L, K in ((20001, 100), (320001, 1000), (1310720, 300), (1310720, 100)):
+        sizes = [need(B, L, 768, K) for B in (1, 31, 32, 127, 128, 256, 257, 511, 512, 513, 2048, 5000, 70000)]
+        if K > 256:
+            assert sizes == sorted(sizes)
+            assert all(s >= need(256, L, 768, K) for s in sizes[5:])
