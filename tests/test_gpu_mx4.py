@@ -420,3 +420,28 @@ def test_topk_of_more_rows_than_the_workspace_has_room_for(dev):
     check(lib().xfc_mx4_topk(x.data_ptr(), 0, d, labels.codes.data_ptr(), labels.scales.data_ptr(), B, L, d, L, K, 8, ev.data_ptr(), ei.data_ptr(), ws.data_ptr(),
                              all_rows, torch.cuda.current_stream().cuda_stream), "xfc_mx4_topk")
     assert torch.equal(v, ev) and torch.equal(i, ei)
+
+
+@pytest.mark.parametrize("B,L,d,K", [(36, 18729, 8, 9), (130, 40961, 72, 10), (300, 41000, 200, 20), (33, 70001, 200, 16), (34, 600003, 8, 256), (260, 100003, 136, 40)])
+def test_topk_with_8_bits_by_maxima(dev, B, L, d, K):
+    """Above 8 labels of enough rows and labels: no logits are written, and the scores that are formed again are those of xfc_forward to the bit, in the
+    order of a stable sort; which holds what test_logits asks of them against 64 bits."""
+    from renee_amd._lib import lib
+
+    assert lib().xfc_mx4_topk_workspace_bytes(B, L, d, K) < B * L
+    x, w, z = _problem(B, L, d, 8, DTYPES[(B + K) % 3], L + K)
+    x[B // 2] = 0
+    if B > 35:
+        x[3, 0] = float("nan")
+    z = O.rounded(x, 8) @ O.rounded(w, 4).t()
+    labels, xd = MX4Labels.from_weight(w.to(dev)), x.to(dev)
+    v, i = labels.topk(xd, K)
+    own = labels.xfc_forward(xd).cpu().double()
+    ev, ei = O.topk(torch.where(torch.isnan(own), -math.inf, own), K)
+    assert torch.equal(v.cpu().double(), ev) and torch.equal(i.cpu(), ei)
+    numbers = ~torch.isnan(x.float()).any(1)
+    tol = (_logit_tolerance(x, w, 8) + z.abs() * 2.0 ** -11)[numbers]
+    chosen = i.cpu()[numbers]
+    assert bool(((v.cpu().double()[numbers] - z[numbers].gather(1, chosen)).abs() <= tol.gather(1, chosen)).all())
+    left = z[numbers].scatter(1, chosen, -math.inf)
+    assert bool((left <= v.cpu().double()[numbers][:, -1:] + tol).all())
