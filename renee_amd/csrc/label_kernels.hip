@@ -300,11 +300,13 @@ static size_t mx_logit_rows_bytes(int64_t rows, int64_t L, int64_t K) {
   return (size_t)round_up((int64_t)logits, 16) + (select_takes_maxima(K, ceil_div(L, LOGIT_BLOCK)) ? (size_t)rows * (size_t)mx_half_maxima(L) * 2 : 0);
 }
 
-// Rows whose logits a call asks for room for: 2 GiB of them, or 512 rows where those are more, whatever the batch.  (Turns of 512 rows / all at once, 768 dims, K =
-// 300: 1024 rows x 1,310,720 labels 1,336 / 1,402 us, 2.8 M 2,715 / 2,949 and 2.8 / 5.7 GB, 600 x 2.8 M 1,760 / 1,755.)
+// Rows whose logits a call asks for room for: all where they are 2 GiB or 512 rows at most, else even turns of that.  (In two turns / all at once, 768 dims, K = 300:
+// 1024 rows x 1,310,720 labels 1,336 / 1,402 us, 1536 2,144 / 2,513, 1024 x 2.8 M 2,715 / 2,949 and 2.8 / 5.9 GB, 600 x 2.8 M 1,760 / 1,755.  Of 768 and 256 rows
+// the first takes 1,426.)
 static int64_t mx_turn_rows(int64_t B, int64_t L, int64_t K) {
-  const int64_t fit = (int64_t)(((size_t)2 << 30) / mx_logit_rows_bytes(256, L, K)) * 256, rows = fit > 512 ? fit : 512;
-  return B < rows ? B : rows;
+  const int64_t fit = (int64_t)(((size_t)2 << 30) / mx_logit_rows_bytes(256, L, K)) * 256, most = fit > 512 ? fit : 512;
+  const int64_t turns = ceil_div(B, most);
+  return turns == 1 ? B : round_up(ceil_div(B, turns), 256);
 }
 
 size_t xfc_mx4_topk_workspace_bytes(int64_t B, int64_t L, int64_t d, int64_t K) {

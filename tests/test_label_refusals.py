@@ -112,7 +112,7 @@ def test_what_gets_no_gradient_may_not_ask_for_one(which):
 
 
 def test_the_logits_of_any_batch_take_bounded_workspace():
-    """What top-K above 8 asks for where it writes logits: all rows up to 512 of them or 2 GiB, no more for more rows, and never less for them."""
+    """What top-K above 8 asks for where it writes logits: all rows up to 512 of them or 2 GiB, no more for more rows, and always what 256 rows take."""
     need = lib().xfc_mx4_topk_workspace_bytes
     per = -(-2812281 // 64) * 64 * 2
     assert need(512, 2812281, 768, 1000) > 512 * per and need(8192, 2812281, 768, 1000) == need(512, 2812281, 768, 1000) < 3 << 30
@@ -122,3 +122,6 @@ def test_the_logits_of_any_batch_take_bounded_workspace():
         if K > 256:
             assert sizes == sorted(sizes)
             assert all(s >= need(256, L, 768, K) for s in sizes[5:])
+    # more rows than fit go in even turns
+    assert need(1024, 1310720, 768, 300) == need(512, 1310720, 768, 300) and need(769, 1310720, 768, 300) == need(512, 1310720, 768, 300)
+    assert need(768, 1310720, 768, 300) > 768 * 1310720 * 2
