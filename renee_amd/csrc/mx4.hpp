@@ -383,7 +383,7 @@ __device__ __forceinline__ void mx_before_maxima(float4v (&acc)[MX_TILES][NT], i
 
 // Bound, with few rows, by the stream of codes: 16 rows x 131,072 x 768 12.8 us for 54 MB of them and 4 of logits, 4.5 TB/s.  With many, logits
 // by the memory that they go to (512 x 1,310,720: 1.34 GB of them beside 0.53 of codes, 455 us at best, 530 to 590 with a warm chip), maxima by the
-// matrix pipes' power: 1024 x 2,812,281 x 768 with 4-bit rows took 990 to 1,080 us, 4.1 to 4.5 PFLOP/s at a clock that falls to 1.7 GHz (registers alone
+// matrix pipes' power: 1024 x 2,812,281 x 768 with 4-bit rows took 990 to 1,080 us, 4.1 to 4.5 PFLOP/s (registers alone
 // reach 7 PFLOP/s on random numbers, 9.6 on zeros); without the fetches it was 200 us less, without the maxima 90: mx4_wide_kernel has such calls now.
 //
 // A workgroup keeps its rows' fragments in the LDS and its waves, which never meet again, stream units of 64 labels past them, straight
