@@ -72,3 +72,45 @@ def test_a_label_matrix_that_requires_grad_gets_none(dev):
     preference_loss(leaf, labels, rowptr, c, r).backward()
     assert labels.grad is None and torch.equal(leaf.grad, preference(x.to(dev), w.to(dev), rowptr, c, r)[2])
     assert not preference_loss(x.to(dev), labels, rowptr, c, r).requires_grad
+
+
+@pytest.mark.parametrize("most", [4, (3, 700)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_gradient_asked_for_in_a_narrow_type_is_rounded_once(dev, dtype, most):
+    """preference(grad_dtype=): rows of one chunk of pairs and of several."""
+    x, w = _problem(40, 60, 72, torch.float32, 51)
+    lists = [t.to(dev) for t in _pairs(40, 60, most, 52)]
+    exact = preference(x.to(dev), w.to(dev), *lists, 0.5, 0.1, 1.5)[2]
+    got = preference(x.to(dev), w.to(dev), *lists, 0.5, 0.1, 1.5, grad_dtype=dtype)[2]
+    assert got.dtype == dtype and torch.equal(got, exact.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_captured_with_a_loss_scale(dev, dtype):
+    """A captured forward and backward pass of narrow embeddings, replayed with new embeddings and scales beside eager calls."""
+    x, w = _problem(20, 300, 128, torch.float32, 53)
+    rowptr, c, r, ref, wt = (t.to(dev) for t in _pairs(20, 300, 7, 54))
+    x, w, scale = x.to(dev), w.to(dev), torch.tensor(65536.0, device=dev)
+    leaf = x.to(dtype).requires_grad_(True)
+
+    def step():
+        (preference_loss(leaf, w, rowptr, c, r, ref, wt, 1e-3) * scale).backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    leaf.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for k in range(4):
+        with torch.no_grad():
+            leaf.copy_(x * (k + 1))
+        scale.fill_(2.0 ** (16 - 4 * k))
+        leaf.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        exact = preference(leaf.detach(), w, rowptr, c, r, ref, wt, 1e-3)[2]
+        assert bool(exact.any()) and torch.equal(leaf.grad, (exact * scale).to(dtype))
