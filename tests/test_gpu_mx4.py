@@ -445,3 +445,27 @@ def test_topk_with_8_bits_by_maxima(dev, B, L, d, K):
     assert bool(((v.cpu().double()[numbers] - z[numbers].gather(1, chosen)).abs() <= tol.gather(1, chosen)).all())
     left = z[numbers].scatter(1, chosen, -math.inf)
     assert bool((left <= v.cpu().double()[numbers][:, -1:] + tol).all())
+
+
+@pytest.mark.parametrize("B,K,bits", [(150, 5, 4), (150, 5, 8), (40, 10, 4), (40, 10, 8), (300, 200, 8)])
+def test_topk_by_maxima_of_four_units_together(dev, B, K, bits):
+    """A million labels and more whose rows do not stay in registers: a wave writes the maxima of four units at once, here with two left over."""
+    L, d = 1_100_100, 64
+    assert -(-L // 64) % 4 == 2
+    g = torch.Generator(device=dev).manual_seed(B + K)
+    w = (torch.randn(L, d, generator=g, device=dev) * 0.02).half()
+    x = torch.randn(B, d, generator=g, device=dev).half()
+    w[-40:] *= 1.25
+    w[L // 3, 3], x[B - 1, d - 1] = float("nan"), float("inf")
+    labels = MX4Labels.from_weight(w)
+    v, i = labels.topk(x, K, embed_bits=bits)
+    z = labels.xfc_forward(x, embed_bits=bits).float()
+    if K <= 8:  # by the fp32 sums, which the logits are the roundings of
+        assert torch.equal(v[:-1].half().float(), z[:-1].gather(1, i[:-1])) and bool((v[:-1, :-1] >= v[:-1, 1:]).all())
+        v = v.half().float()
+    z = torch.where(torch.isnan(z), -math.inf, z)
+    for r0 in range(0, B, 64):
+        ev, ei = (t[:, :K] for t in torch.sort(z[r0:r0 + 64], dim=1, descending=True, stable=True))
+        assert torch.equal(v[r0:r0 + 64], ev)
+        if K > 8:
+            assert torch.equal(i[r0:r0 + 64], ei)
